@@ -177,6 +177,77 @@ int attn_decode_f16_noalloc(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_k
 int attn_prefill_f16(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0,
                      uint32_t rows, const float *q, uint32_t q_row_stride, const uint16_t *kc, const uint16_t *vc,
                      uint64_t token_stride, uint64_t head_stride, float *out, uint32_t out_row_stride);
+/* ---- An 8-bit KV cache, and attention of a batch that shares a prefix.  No
+ * reference counterpart (its cache is f32 and it decodes one sequence).
+ *
+ * A cache is a K and a V buffer of rows of head_dim (64 or 128) elements:
+ * element (s, t, h, d) of sequence s, token t, KV head h at s*seq_stride +
+ * t*token_stride + h*head_stride + d.  fp16 caches are attn_decode_f16's
+ * (strides multiples of 8).  8-bit caches hold e4m3 codes (strides multiples
+ * of head_dim) and, in k_scales and v_scales, one E8M0 byte for each row at
+ * the row's element offset / head_dim: a value is code * 2^(byte - 127).  Byte
+ * 255 makes the whole row NaN; codes 0x7F and 0xFF (NaN) are not used, and
+ * what a buffer holds past the tokens that a call names does not matter.  All
+ * buffers, and rows of q, k, v and out, 16-byte aligned (scales: any).
+ *
+ * These calls share nothing: each works in the caller's workspace (16-byte
+ * aligned, of any content, at least the bytes that the call's _workspace
+ * function says for the same arguments; 0 bytes may be NULL), so calls on
+ * several streams need a workspace each, and so do captured graphs that may
+ * run at once.  They only launch kernels and may be captured. */
+/* New rows of K and V (f32; row r at k + r*k_row_stride, v + r*v_row_stride,
+ * [n_kv_heads][head_dim]) into a cache, fp16 (RNE) or 8 bits: for each row and
+ * KV head the smallest scale 2^e, e >= -127, with which the largest magnitude
+ * is at most 448, codes rounded to nearest even; a row of zeros gets byte 0, a
+ * row with an infinity or NaN byte 255 and codes 0.  positions NULL: row r is
+ * token pos0 + r of one sequence (seq_stride unused; past `capacity` tokens
+ * RFP4_E_KV_OVERFLOW).  Else row r is token positions[r] (device memory) of
+ * sequence r, and a row whose position is not below `capacity` is left out
+ * (padding).  Strides must keep rows apart (RFP4_E_SHAPE). */
+int kv_append_rows_f16(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0,
+                       const uint32_t *positions, const float *k, uint32_t k_row_stride, const float *v,
+                       uint32_t v_row_stride, uint16_t *kc, uint16_t *vc, uint64_t seq_stride, uint64_t token_stride,
+                       uint64_t head_stride, uint32_t capacity);
+int kv_append_rows_fp8(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0,
+                       const uint32_t *positions, const float *k, uint32_t k_row_stride, const float *v,
+                       uint32_t v_row_stride, uint8_t *kc, uint8_t *k_scales, uint8_t *vc, uint8_t *v_scales,
+                       uint64_t seq_stride, uint64_t token_stride, uint64_t head_stride, uint32_t capacity);
+/* attn_decode_f16 over an 8-bit cache: one query row, `seq` >= 1 tokens. */
+size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq);
+int attn_decode_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq,
+                    const float *q, const uint8_t *kc, const uint8_t *k_scales, const uint8_t *vc,
+                    const uint8_t *v_scales, uint64_t token_stride, uint64_t head_stride, void *workspace,
+                    size_t workspace_bytes, float *out);
+/* attn_prefill_f16 over an 8-bit cache: causal rows at positions pos0 ..
+ * pos0+rows-1, their own k and v already in it. */
+size_t attn_prefill_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows);
+int attn_prefill_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0,
+                     uint32_t rows, const float *q, uint32_t q_row_stride, const uint8_t *kc, const uint8_t *k_scales,
+                     const uint8_t *vc, const uint8_t *v_scales, uint64_t token_stride, uint64_t head_stride,
+                     void *workspace, size_t workspace_bytes, float *out, uint32_t out_row_stride);
+/* Decode attention of a batch whose sequences share their first tokens: row b
+ * (q + b*q_row_stride) attends to the `prefix` tokens of the shared cache (pk,
+ * pv; read once for the batch, not once for each row) and then to the first
+ * suffix_lens[b] (device memory; at most max_suffix count) tokens of its own
+ * cache, sequence b of sk, sv.  Either part may be empty (its pointers are then
+ * not looked at); a row without any token is 0.  The shared cache may be an
+ * engine's (llama_engine_kv).  The workspace is the same for both types. */
+size_t attn_decode_prefix_workspace(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                                    uint32_t prefix, uint32_t max_suffix);
+int attn_decode_prefix_f16(rfp4_stream_t stream, uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads,
+                           uint32_t head_dim, const float *q, uint32_t q_row_stride, uint32_t prefix, const uint16_t *pk,
+                           const uint16_t *pv, uint64_t p_token_stride, uint64_t p_head_stride, uint32_t max_suffix,
+                           const uint32_t *suffix_lens, const uint16_t *sk, const uint16_t *sv, uint64_t s_seq_stride,
+                           uint64_t s_token_stride, uint64_t s_head_stride, void *workspace, size_t workspace_bytes,
+                           float *out, uint32_t out_row_stride);
+int attn_decode_prefix_fp8(rfp4_stream_t stream, uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads,
+                           uint32_t head_dim, const float *q, uint32_t q_row_stride, uint32_t prefix, const uint8_t *pk,
+                           const uint8_t *pk_scales, const uint8_t *pv, const uint8_t *pv_scales,
+                           uint64_t p_token_stride, uint64_t p_head_stride, uint32_t max_suffix,
+                           const uint32_t *suffix_lens, const uint8_t *sk, const uint8_t *sk_scales, const uint8_t *sv,
+                           const uint8_t *sv_scales, uint64_t s_seq_stride, uint64_t s_token_stride,
+                           uint64_t s_head_stride, void *workspace, size_t workspace_bytes, float *out,
+                           uint32_t out_row_stride);
 /* swiglu(n, gate, up, out): llama_run/src/main.rs:244-252 */
 int swiglu(rfp4_stream_t stream, uint32_t n, const float *gate, const float *up, float *out);
 /* residual(n, y, x): x += y, llama_run/src/main.rs:254-261 */

@@ -1,0 +1,291 @@
+// C-ABI entry points of the 8-bit KV cache, of the attention over it, and of
+// attention of a batch that shares a prefix (include/rfp4.h): argument checks
+// and launch plans.  Nothing of the library's is shared between calls: split
+// states live in the caller's workspace.
+#include "runtime.h"
+
+#include <algorithm>
+#include <cstdio>
+
+using namespace rfp4;
+
+namespace {
+
+bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// Keys and rows a call may have: 32-bit key and row counts with room for a
+// block past the end.
+constexpr uint64_t kMaxKeys = (uint64_t)1 << 31;
+constexpr uint64_t kMaxStride = (uint64_t)1 << 48; // elements
+
+struct Cache {
+    const void *k, *v;
+    const uint8_t *ks, *vs;
+    uint64_t ts, hs, ss;
+};
+
+// A cache of `what`'s: pointers, 16-byte aligned rows, and for the 8-bit one
+// strides of whole rows (a row's scale is at its element offset / head_dim).
+int check_cache(const char *what, const Cache &c, bool fp8, uint32_t hd)
+{
+    if (!c.k || !c.v || (fp8 && (!c.ks || !c.vs))) return set_error(RFP4_E_INVALID, "%s: null cache pointer", what);
+    const uint64_t unit = fp8 ? hd : 8u;
+    if (!aligned(c.k, 16) || !aligned(c.v, 16) || c.ts % unit || c.hs % unit || c.ss % unit)
+        return set_error(RFP4_E_ALIGN, "%s: cache rows must start 16-byte aligned, strides (%llu, %llu, %llu) be multiples of %llu", what,
+                         (unsigned long long)c.ss, (unsigned long long)c.ts, (unsigned long long)c.hs, (unsigned long long)unit);
+    if (c.ts >= kMaxStride || c.hs >= kMaxStride || c.ss >= kMaxStride) return set_error(RFP4_E_SHAPE, "%s: stride over 2^48", what);
+    return RFP4_OK;
+}
+
+int check_heads(const char *what, uint32_t nh, uint32_t nkv, uint32_t hd)
+{
+    if (hd != 64 && hd != 128) return set_error(RFP4_E_SHAPE, "%s: head_dim %u unsupported (64 or 128)", what, hd);
+    if (nkv == 0 || nh == 0 || nh % nkv || nh / nkv > 8)
+        return set_error(RFP4_E_SHAPE, "%s: %u query heads over %u KV heads (group of at most 8)", what, nh, nkv);
+    return RFP4_OK;
+}
+
+int check_rows(const char *what, const float *q, uint32_t q_rs, const float *out, uint32_t out_rs, uint32_t rows, uint32_t nh, uint32_t hd)
+{
+    if (!q || !out) return set_error(RFP4_E_INVALID, "%s: null pointer", what);
+    if (!aligned(q, 16) || !aligned(out, 16) || q_rs % 4u || out_rs % 4u)
+        return set_error(RFP4_E_ALIGN, "%s: q and out rows must start 16-byte aligned", what);
+    if ((uint64_t)nh * hd > UINT32_MAX || (rows > 1 && (q_rs < nh * hd || out_rs < nh * hd)))
+        return set_error(RFP4_E_SHAPE, "%s: row strides %u, %u < %u heads x %u", what, q_rs, out_rs, nh, hd);
+    return RFP4_OK;
+}
+
+// How a call is cut: the kernel by its query rows of a KV head, the keys into
+// splits.
+struct Plan {
+    int mt, wk;
+    uint32_t tiles0, splits0, chunk0, splits1, chunk1;
+    uint32_t splits() const { return splits0 + splits1; }
+};
+
+// Workgroups that fill the chip: two of 4 waves on each of its 256 CUs.
+constexpr uint64_t kWorkgroups = 512;
+
+void cut(uint64_t keys, uint64_t others, uint64_t least, uint32_t *splits, uint32_t *chunk)
+{
+    // as many splits as the other dimensions leave workgroups for, of at least `least` keys, whole blocks of 4 waves
+    uint64_t n = std::max<uint64_t>(1, kWorkgroups / std::max<uint64_t>(1, others));
+    n = std::max<uint64_t>(1, std::min(n, keys / least));
+    const uint64_t c = ((keys + n - 1) / n + 127) / 128 * 128;
+    *chunk = (uint32_t)c;
+    *splits = (uint32_t)((keys + c - 1) / c);
+}
+
+Plan plan(uint32_t nkv, uint32_t group, uint32_t rows, uint64_t len0, uint64_t cap1)
+{
+    Plan p{};
+    const uint64_t flat = (uint64_t)rows * group;
+    if (flat <= 16) {
+        p.mt = 1;
+        p.wk = 4;
+    } else {
+        p.mt = 2;
+        p.wk = 1;
+    }
+    const uint64_t rw = 16u * (uint64_t)p.mt * (4u / (uint64_t)p.wk);
+    if (len0) {
+        p.tiles0 = (uint32_t)((flat + rw - 1) / rw);
+        cut(len0, (uint64_t)p.tiles0 * nkv, 256, &p.splits0, &p.chunk0);
+    }
+    if (cap1) cut(cap1, (uint64_t)rows * nkv, 256, &p.splits1, &p.chunk1);
+    return p;
+}
+
+size_t plan_bytes(const Plan &p, uint32_t rows, uint32_t nh, uint32_t hd)
+{
+    return p.splits() > 1 ? (size_t)rows * nh * p.splits() * (hd + 4) * sizeof(float) : 0;
+}
+
+int run(const char *what, const Plan &p, AttnRowsArgs &a, bool fp8, uint32_t hd, void *workspace, size_t workspace_bytes, hipStream_t s)
+{
+    const size_t need = plan_bytes(p, a.rows, a.n_heads, hd);
+    if (need && !workspace) return set_error(RFP4_E_INVALID, "%s: null workspace (%zu bytes)", what, need);
+    if (need && !aligned(workspace, 16)) return set_error(RFP4_E_ALIGN, "%s: workspace must be 16-byte aligned", what);
+    if (need > workspace_bytes)
+        return set_error(RFP4_E_CAPACITY, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+    a.part = (float *)workspace;
+    a.group = a.n_heads / a.n_kv_heads;
+    a.tiles0 = p.tiles0;
+    a.splits0 = p.splits0;
+    a.chunk0 = p.chunk0;
+    a.splits1 = p.splits1;
+    a.chunk1 = p.chunk1;
+    const uint64_t items = ((uint64_t)p.tiles0 * p.splits0 + (uint64_t)a.rows * p.splits1) * a.n_kv_heads;
+    const uint64_t merges = (uint64_t)a.rows * a.n_heads;
+    if (std::max(items, merges) > ((uint64_t)1 << 23))
+        return set_error(RFP4_E_CAPACITY, "%s: %llu workgroups (at most 2^23)", what, (unsigned long long)std::max(items, merges));
+    char name[64];
+    if (items) {
+        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_t%dk%d", hd, fp8 ? "fp8" : "f16", p.mt, p.wk);
+        if (int rc = launch(name, dim3((unsigned)items), dim3(256), s, &a)) return rc;
+    }
+    if (p.splits() == 1) return RFP4_OK;
+    // the splits' states, or the zeros of rows that have no keys at all
+    return launch(hd == 64 ? "rfp4_attn_rows_merge_hd64" : "rfp4_attn_rows_merge_hd128", dim3((unsigned)merges), dim3(256), s, &a);
+}
+
+int append_rows(const char *what, bool fp8, hipStream_t s, uint32_t rows, uint32_t nkv, uint32_t hd, uint32_t pos0, const uint32_t *positions,
+                const float *k, uint32_t k_rs, const float *v, uint32_t v_rs, void *kc, uint8_t *ks, void *vc, uint8_t *vs, uint64_t ss,
+                uint64_t ts, uint64_t hs, uint32_t capacity)
+{
+    if (hd != 64 && hd != 128) return set_error(RFP4_E_SHAPE, "%s: head_dim %u unsupported (64 or 128)", what, hd);
+    if (nkv == 0) return set_error(RFP4_E_SHAPE, "%s: n_kv_heads must be > 0", what);
+    if (rows == 0) return RFP4_OK;
+    if (!k || !v) return set_error(RFP4_E_INVALID, "%s: null pointer", what);
+    const Cache c{kc, vc, ks, vs, ts, hs, positions ? ss : 0};
+    if (int rc = check_cache(what, c, fp8, hd)) return rc;
+    if (!aligned(k, 16) || !aligned(v, 16) || k_rs % 4u || v_rs % 4u)
+        return set_error(RFP4_E_ALIGN, "%s: k and v rows must start 16-byte aligned", what);
+    if ((uint64_t)nkv * hd > UINT32_MAX || (rows > 1 && (k_rs < nkv * hd || v_rs < nkv * hd)))
+        return set_error(RFP4_E_SHAPE, "%s: row strides %u, %u < %u heads x %u", what, k_rs, v_rs, nkv, hd);
+    if (!positions && (uint64_t)pos0 + rows > capacity)
+        return set_error(RFP4_E_KV_OVERFLOW, "%s: positions %u .. %llu of a cache of %u", what, pos0, (unsigned long long)pos0 + rows - 1, capacity);
+    // no two rows may share memory: by stride, each dimension spans what the smaller ones cover
+    struct { uint64_t n, stride; } dim[3] = {{capacity, ts}, {nkv, hs}, {positions ? rows : 1u, ss}};
+    std::sort(dim, dim + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });
+    unsigned __int128 span = hd;
+    for (const auto &d : dim) {
+        if (d.n <= 1) continue;
+        if (d.stride < span) return set_error(RFP4_E_SHAPE, "%s: strides (%llu, %llu, %llu) make cache rows overlap", what, (unsigned long long)ss,
+                                              (unsigned long long)ts, (unsigned long long)hs);
+        span += (unsigned __int128)d.stride * (d.n - 1);
+    }
+    const uint64_t units = (uint64_t)rows * 2u * nkv, per = 256u / (hd / 8u);
+    if (units > ((uint64_t)1 << 27)) return set_error(RFP4_E_CAPACITY, "%s: %u rows of %u heads in one call", what, rows, nkv);
+    KvRowsArgs a{k, v, kc, vc, ks, vs, positions, positions ? ss : 0, ts, hs, k_rs, v_rs, rows, nkv, pos0, capacity};
+    char name[48];
+    snprintf(name, sizeof name, "rfp4_kv_rows_hd%u_%s", hd, fp8 ? "fp8" : "f16");
+    return launch(name, dim3((unsigned)((units + per - 1) / per)), dim3(256), s, &a);
+}
+
+int causal(const char *what, hipStream_t s, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t pos0, uint32_t rows, const float *q, uint32_t q_rs,
+           const Cache &c, void *workspace, size_t workspace_bytes, float *out, uint32_t out_rs)
+{
+    if (int rc = check_heads(what, nh, nkv, hd)) return rc;
+    if (rows == 0) return RFP4_OK;
+    if (int rc = check_rows(what, q, q_rs, out, out_rs, rows, nh, hd)) return rc;
+    if (int rc = check_cache(what, c, true, hd)) return rc;
+    const uint64_t keys = (uint64_t)pos0 + rows;
+    if (keys > kMaxKeys || (uint64_t)rows * nh > kMaxKeys) return set_error(RFP4_E_SHAPE, "%s: %llu keys, %u rows", what, (unsigned long long)keys, rows);
+    AttnRowsArgs a{};
+    a.q = q; a.out = out;
+    a.k0 = c.k; a.v0 = c.v; a.ks0 = c.ks; a.vs0 = c.vs;
+    a.ts0 = c.ts; a.hs0 = c.hs;
+    a.q_rs = q_rs; a.out_rs = out_rs;
+    a.n_heads = nh; a.n_kv_heads = nkv;
+    a.rows = rows; a.causal = 1; a.pos0 = pos0; a.len0 = (uint32_t)keys;
+    return run(what, plan(nkv, nh / nkv, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
+}
+
+int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint32_t nh, uint32_t nkv, uint32_t hd, const float *q, uint32_t q_rs,
+                uint32_t prefix, const Cache &p, uint32_t max_suffix, const uint32_t *lens, const Cache &own, void *workspace,
+                size_t workspace_bytes, float *out, uint32_t out_rs)
+{
+    if (int rc = check_heads(what, nh, nkv, hd)) return rc;
+    if (batch == 0) return RFP4_OK;
+    if (int rc = check_rows(what, q, q_rs, out, out_rs, batch, nh, hd)) return rc;
+    if (prefix)
+        if (int rc = check_cache(what, p, fp8, hd)) return rc;
+    if (max_suffix) {
+        if (!lens) return set_error(RFP4_E_INVALID, "%s: null suffix lengths", what);
+        if (int rc = check_cache(what, own, fp8, hd)) return rc;
+    }
+    if (prefix > kMaxKeys || max_suffix > kMaxKeys || (uint64_t)batch * nh > kMaxKeys)
+        return set_error(RFP4_E_SHAPE, "%s: prefix %u, suffix %u, batch %u", what, prefix, max_suffix, batch);
+    AttnRowsArgs a{};
+    a.q = q; a.out = out;
+    a.k0 = p.k; a.v0 = p.v; a.ks0 = p.ks; a.vs0 = p.vs;
+    a.ts0 = p.ts; a.hs0 = p.hs;
+    a.k1 = own.k; a.v1 = own.v; a.ks1 = own.ks; a.vs1 = own.vs;
+    a.ts1 = own.ts; a.hs1 = own.hs; a.ss1 = own.ss;
+    a.lens = lens;
+    a.q_rs = q_rs; a.out_rs = out_rs;
+    a.n_heads = nh; a.n_kv_heads = nkv;
+    a.rows = batch; a.len0 = prefix; a.cap1 = max_suffix;
+    return run(what, plan(nkv, nh / nkv, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
+}
+
+} // namespace
+
+extern "C" {
+
+int kv_append_rows_f16(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, const uint32_t *positions,
+                       const float *k, uint32_t k_row_stride, const float *v, uint32_t v_row_stride, uint16_t *kc, uint16_t *vc,
+                       uint64_t seq_stride, uint64_t token_stride, uint64_t head_stride, uint32_t capacity)
+{
+    return append_rows("kv_append_rows_f16", false, (hipStream_t)stream, rows, n_kv_heads, head_dim, pos0, positions, k, k_row_stride, v,
+                       v_row_stride, kc, nullptr, vc, nullptr, seq_stride, token_stride, head_stride, capacity);
+}
+
+int kv_append_rows_fp8(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, const uint32_t *positions,
+                       const float *k, uint32_t k_row_stride, const float *v, uint32_t v_row_stride, uint8_t *kc, uint8_t *k_scales, uint8_t *vc,
+                       uint8_t *v_scales, uint64_t seq_stride, uint64_t token_stride, uint64_t head_stride, uint32_t capacity)
+{
+    return append_rows("kv_append_rows_fp8", true, (hipStream_t)stream, rows, n_kv_heads, head_dim, pos0, positions, k, k_row_stride, v,
+                       v_row_stride, kc, k_scales, vc, v_scales, seq_stride, token_stride, head_stride, capacity);
+}
+
+size_t attn_prefill_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows)
+{
+    if (check_heads("attn_prefill_fp8_workspace", n_heads, n_kv_heads, head_dim) || rows == 0) return 0;
+    return plan_bytes(plan(n_kv_heads, n_heads / n_kv_heads, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
+}
+
+size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq)
+{
+    return seq ? attn_prefill_fp8_workspace(n_heads, n_kv_heads, head_dim, seq - 1u, 1) : 0;
+}
+
+size_t attn_decode_prefix_workspace(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t prefix, uint32_t max_suffix)
+{
+    if (check_heads("attn_decode_prefix_workspace", n_heads, n_kv_heads, head_dim) || batch == 0) return 0;
+    return plan_bytes(plan(n_kv_heads, n_heads / n_kv_heads, batch, prefix, max_suffix), batch, n_heads, head_dim);
+}
+
+int attn_decode_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq, const float *q,
+                    const uint8_t *kc, const uint8_t *k_scales, const uint8_t *vc, const uint8_t *v_scales, uint64_t token_stride,
+                    uint64_t head_stride, void *workspace, size_t workspace_bytes, float *out)
+{
+    if (seq == 0) return set_error(RFP4_E_SHAPE, "attn_decode_fp8: seq must be >= 1");
+    return causal("attn_decode_fp8", (hipStream_t)stream, n_heads, n_kv_heads, head_dim, seq - 1u, 1, q, 0,
+                  Cache{kc, vc, k_scales, v_scales, token_stride, head_stride, 0}, workspace, workspace_bytes, out, 0);
+}
+
+int attn_prefill_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows, const float *q,
+                     uint32_t q_row_stride, const uint8_t *kc, const uint8_t *k_scales, const uint8_t *vc, const uint8_t *v_scales,
+                     uint64_t token_stride, uint64_t head_stride, void *workspace, size_t workspace_bytes, float *out, uint32_t out_row_stride)
+{
+    return causal("attn_prefill_fp8", (hipStream_t)stream, n_heads, n_kv_heads, head_dim, pos0, rows, q, q_row_stride,
+                  Cache{kc, vc, k_scales, v_scales, token_stride, head_stride, 0}, workspace, workspace_bytes, out, out_row_stride);
+}
+
+int attn_decode_prefix_f16(rfp4_stream_t stream, uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float *q,
+                           uint32_t q_row_stride, uint32_t prefix, const uint16_t *pk, const uint16_t *pv, uint64_t p_token_stride,
+                           uint64_t p_head_stride, uint32_t max_suffix, const uint32_t *suffix_lens, const uint16_t *sk, const uint16_t *sv,
+                           uint64_t s_seq_stride, uint64_t s_token_stride, uint64_t s_head_stride, void *workspace, size_t workspace_bytes,
+                           float *out, uint32_t out_row_stride)
+{
+    return prefix_rows("attn_decode_prefix_f16", false, (hipStream_t)stream, batch, n_heads, n_kv_heads, head_dim, q, q_row_stride, prefix,
+                       Cache{pk, pv, nullptr, nullptr, p_token_stride, p_head_stride, 0}, max_suffix, suffix_lens,
+                       Cache{sk, sv, nullptr, nullptr, s_token_stride, s_head_stride, s_seq_stride}, workspace, workspace_bytes, out, out_row_stride);
+}
+
+int attn_decode_prefix_fp8(rfp4_stream_t stream, uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, const float *q,
+                           uint32_t q_row_stride, uint32_t prefix, const uint8_t *pk, const uint8_t *pk_scales, const uint8_t *pv,
+                           const uint8_t *pv_scales, uint64_t p_token_stride, uint64_t p_head_stride, uint32_t max_suffix,
+                           const uint32_t *suffix_lens, const uint8_t *sk, const uint8_t *sk_scales, const uint8_t *sv, const uint8_t *sv_scales,
+                           uint64_t s_seq_stride, uint64_t s_token_stride, uint64_t s_head_stride, void *workspace, size_t workspace_bytes,
+                           float *out, uint32_t out_row_stride)
+{
+    return prefix_rows("attn_decode_prefix_fp8", true, (hipStream_t)stream, batch, n_heads, n_kv_heads, head_dim, q, q_row_stride, prefix,
+                       Cache{pk, pv, pk_scales, pv_scales, p_token_stride, p_head_stride, 0}, max_suffix, suffix_lens,
+                       Cache{sk, sv, sk_scales, sv_scales, s_token_stride, s_head_stride, s_seq_stride}, workspace, workspace_bytes, out,
+                       out_row_stride);
+}
+
+} // extern "C"

@@ -12,6 +12,8 @@
 #include "device/gemm_rows.h"
 #include "device/prefill.h"
 #include "device/attn_prefill.h"
+#include "device/kv_rows.h"
+#include "device/attn_rows.h"
 #include "device/persist.h"
 #include "device/qkva.h"
 
@@ -175,6 +177,20 @@ QKVA_KERNELS(128, 2, 4, 4, )
 QKVA_KERNELS(64, 1, 1, 8, _r1)
 K256 void rfp4_attn_merge_hd64(AttnArgs a) { attn_merge_body<64>(a); }
 K256 void rfp4_attn_merge_hd128(AttnArgs a) { attn_merge_body<128>(a); }
+
+// ---- the 8-bit cache, and attention of rows and batches
+// (device/kv_rows.h, device/attn_rows.h): rfp4_attn_rows_hd<HD>_<type>_t<MT>k<WK>,
+// 16 MT (4 / WK) query rows and WK key groups per workgroup (attn_rows.cpp)
+#define ATTN_ROWS_KERNELS(HD, NAME, F8) \
+    K256 void rfp4_kv_rows_hd##HD##_##NAME(KvRowsArgs a) { kv_rows_body<HD, F8>(a); } \
+    K256 void rfp4_attn_rows_hd##HD##_##NAME##_t1k4(AttnRowsArgs a) { attn_rows_body<HD, F8, 1, 4>(a); } \
+    K256 void rfp4_attn_rows_hd##HD##_##NAME##_t2k1(AttnRowsArgs a) { attn_rows_body<HD, F8, 2, 1>(a); }
+ATTN_ROWS_KERNELS(64, fp8, true)
+ATTN_ROWS_KERNELS(64, f16, false)
+ATTN_ROWS_KERNELS(128, fp8, true)
+ATTN_ROWS_KERNELS(128, f16, false)
+K256 void rfp4_attn_rows_merge_hd64(AttnRowsArgs a) { attn_rows_merge_body<64>(a); }
+K256 void rfp4_attn_rows_merge_hd128(AttnRowsArgs a) { attn_rows_merge_body<128>(a); }
 
 // ---- misc
 K256 void rfp4_fill(FillArgs a) { fill_body(a); }

@@ -145,6 +145,35 @@ typedef struct AttnPrefillArgs {
     uint8_t *q_codes, *q_scales, *q_scales_t;
 } AttnPrefillArgs;
 
+// New K and V rows into a cache (device/kv_rows.h): row r of sequence `r` at
+// positions[r], or, without positions, of one sequence at pos0 + r; rows at or
+// past `capacity` are left out.
+typedef struct KvRowsArgs {
+    const float *k, *v;        // row r: + r*k_rs, r*v_rs, [n_kv_heads][head_dim]
+    void *kc, *vc;             // element (s, t, h, d) at s*ss + t*ts + h*hs + d: fp16, or e4m3 codes
+    uint8_t *ks, *vs;          // e4m3: the row's scale byte at (s*ss + t*ts + h*hs) / head_dim
+    const uint32_t *positions; // null: one sequence
+    uint64_t ss, ts, hs;
+    uint32_t k_rs, v_rs, rows, n_kv_heads, pos0, capacity;
+} KvRowsArgs;
+
+// Attention of query rows over a cache of 8 bits or fp16 (device/attn_rows.h).
+// Keys: `0` those that every row may see (len0 of them; causal: row i the
+// first pos0 + i + 1), `1` each row's own, the first min(lens[i], cap1).
+typedef struct AttnRowsArgs {
+    const float *q;            // row i: q + i*q_rs, [n_heads][head_dim]
+    float *out;                // row i: out + i*out_rs
+    float *part;               // [rows][n_heads][splits0 + splits1][head_dim + 4] = (m, l, -, -, acc)
+    const void *k0, *v0, *k1, *v1;          // element (t, h, d) at t*ts + h*hs + d; of `1` in row i + i*ss1
+    const uint8_t *ks0, *vs0, *ks1, *vs1;   // e4m3: scale bytes at that offset / head_dim
+    uint64_t ts0, hs0, ts1, hs1, ss1;
+    const uint32_t *lens;
+    uint32_t q_rs, out_rs, n_heads, n_kv_heads, group, rows;
+    uint32_t causal, pos0, len0, cap1;
+    uint32_t tiles0, splits0, chunk0;       // row tiles and key splits of `0`
+    uint32_t splits1, chunk1;               // key splits of each row of `1`
+} AttnRowsArgs;
+
 // Batched prefill row kernels (device/prefill.h).
 typedef struct RowsArgs {
     const float *x;          // rmsnorm: rows [rows][k]; swiglu: gate|up rows [rows][2k]

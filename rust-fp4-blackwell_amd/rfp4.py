@@ -95,6 +95,17 @@ _SIGS = {
     "attn_decode_f16": (I32, [P, U32, U32, U32, U32, P, P, P, U64, U64, P]),
     "attn_decode_f16_noalloc": (I32, [P, U32, U32, U32, U32, P, P, P, U64, U64, P]),
     "attn_prefill_f16": (I32, [P, U32, U32, U32, U32, U32, P, U32, P, P, U64, U64, P, U32]),
+    "kv_append_rows_f16": (I32, [P, U32, U32, U32, U32, P, P, U32, P, U32, P, P, U64, U64, U64, U32]),
+    "kv_append_rows_fp8": (I32, [P, U32, U32, U32, U32, P, P, U32, P, U32, P, P, P, P, U64, U64, U64, U32]),
+    "attn_decode_fp8_workspace": (SZ, [U32, U32, U32, U32]),
+    "attn_decode_fp8": (I32, [P, U32, U32, U32, U32, P, P, P, P, P, U64, U64, P, SZ, P]),
+    "attn_prefill_fp8_workspace": (SZ, [U32, U32, U32, U32, U32]),
+    "attn_prefill_fp8": (I32, [P, U32, U32, U32, U32, U32, P, U32, P, P, P, P, U64, U64, P, SZ, P, U32]),
+    "attn_decode_prefix_workspace": (SZ, [U32, U32, U32, U32, U32, U32]),
+    "attn_decode_prefix_f16": (I32, [P, U32, U32, U32, U32, P, U32, U32, P, P, U64, U64, U32, P, P, P, U64, U64, U64, P, SZ,
+                                     P, U32]),
+    "attn_decode_prefix_fp8": (I32, [P, U32, U32, U32, U32, P, U32, U32, P, P, P, P, U64, U64, U32, P, P, P, P, P, U64, U64,
+                                     U64, P, SZ, P, U32]),
     "swiglu": (I32, [P, U32, P, P, P]),
     "residual": (I32, [P, U32, P, P]),
     "argmax": (I32, [P, U32, P, P]),
@@ -447,6 +458,66 @@ def attn_prefill_f16(stream, n_heads, n_kv_heads, head_dim, pos0, rows, q, q_row
                      head_stride, out, out_row_stride):
     check(load().attn_prefill_f16(_s(stream), n_heads, n_kv_heads, head_dim, pos0, rows, _p(q), q_row_stride, _p(kc),
                                   _p(vc), token_stride, head_stride, _p(out), out_row_stride))
+
+
+def kv_append_rows_f16(stream, rows, n_kv_heads, head_dim, pos0, positions, k, k_row_stride, v, v_row_stride, kc, vc,
+                       seq_stride, token_stride, head_stride, capacity):
+    """Rows of K and V (f32) into an fp16 cache: at pos0 .. of one sequence, or row r at positions[r] of sequence r."""
+    check(load().kv_append_rows_f16(_s(stream), rows, n_kv_heads, head_dim, pos0, _p(positions), _p(k), k_row_stride,
+                                    _p(v), v_row_stride, _p(kc), _p(vc), seq_stride, token_stride, head_stride, capacity))
+
+
+def kv_append_rows_fp8(stream, rows, n_kv_heads, head_dim, pos0, positions, k, k_row_stride, v, v_row_stride, kc, k_scales,
+                       vc, v_scales, seq_stride, token_stride, head_stride, capacity):
+    """kv_append_rows_f16 into e4m3 codes with one E8M0 scale for each row and KV head."""
+    check(load().kv_append_rows_fp8(_s(stream), rows, n_kv_heads, head_dim, pos0, _p(positions), _p(k), k_row_stride,
+                                    _p(v), v_row_stride, _p(kc), _p(k_scales), _p(vc), _p(v_scales), seq_stride,
+                                    token_stride, head_stride, capacity))
+
+
+def attn_decode_fp8_workspace(n_heads, n_kv_heads, head_dim, seq) -> int:
+    return int(load().attn_decode_fp8_workspace(n_heads, n_kv_heads, head_dim, seq))
+
+
+def attn_decode_fp8(stream, n_heads, n_kv_heads, head_dim, seq, q, kc, k_scales, vc, v_scales, token_stride, head_stride,
+                    workspace, workspace_bytes, out):
+    check(load().attn_decode_fp8(_s(stream), n_heads, n_kv_heads, head_dim, seq, _p(q), _p(kc), _p(k_scales), _p(vc),
+                                 _p(v_scales), token_stride, head_stride, _p(workspace), workspace_bytes, _p(out)))
+
+
+def attn_prefill_fp8_workspace(n_heads, n_kv_heads, head_dim, pos0, rows) -> int:
+    return int(load().attn_prefill_fp8_workspace(n_heads, n_kv_heads, head_dim, pos0, rows))
+
+
+def attn_prefill_fp8(stream, n_heads, n_kv_heads, head_dim, pos0, rows, q, q_row_stride, kc, k_scales, vc, v_scales,
+                     token_stride, head_stride, workspace, workspace_bytes, out, out_row_stride):
+    check(load().attn_prefill_fp8(_s(stream), n_heads, n_kv_heads, head_dim, pos0, rows, _p(q), q_row_stride, _p(kc),
+                                  _p(k_scales), _p(vc), _p(v_scales), token_stride, head_stride, _p(workspace),
+                                  workspace_bytes, _p(out), out_row_stride))
+
+
+def attn_decode_prefix_workspace(batch, n_heads, n_kv_heads, head_dim, prefix, max_suffix) -> int:
+    return int(load().attn_decode_prefix_workspace(batch, n_heads, n_kv_heads, head_dim, prefix, max_suffix))
+
+
+def attn_decode_prefix_f16(stream, batch, n_heads, n_kv_heads, head_dim, q, q_row_stride, prefix, pk, pv, p_token_stride,
+                           p_head_stride, max_suffix, suffix_lens, sk, sv, s_seq_stride, s_token_stride, s_head_stride,
+                           workspace, workspace_bytes, out, out_row_stride):
+    """One query row for each sequence of a batch over `prefix` shared tokens, then suffix_lens[b] tokens of its own."""
+    check(load().attn_decode_prefix_f16(_s(stream), batch, n_heads, n_kv_heads, head_dim, _p(q), q_row_stride, prefix,
+                                        _p(pk), _p(pv), p_token_stride, p_head_stride, max_suffix, _p(suffix_lens),
+                                        _p(sk), _p(sv), s_seq_stride, s_token_stride, s_head_stride, _p(workspace),
+                                        workspace_bytes, _p(out), out_row_stride))
+
+
+def attn_decode_prefix_fp8(stream, batch, n_heads, n_kv_heads, head_dim, q, q_row_stride, prefix, pk, pk_scales, pv,
+                           pv_scales, p_token_stride, p_head_stride, max_suffix, suffix_lens, sk, sk_scales, sv, sv_scales,
+                           s_seq_stride, s_token_stride, s_head_stride, workspace, workspace_bytes, out, out_row_stride):
+    check(load().attn_decode_prefix_fp8(_s(stream), batch, n_heads, n_kv_heads, head_dim, _p(q), q_row_stride, prefix,
+                                        _p(pk), _p(pk_scales), _p(pv), _p(pv_scales), p_token_stride, p_head_stride,
+                                        max_suffix, _p(suffix_lens), _p(sk), _p(sk_scales), _p(sv), _p(sv_scales),
+                                        s_seq_stride, s_token_stride, s_head_stride, _p(workspace), workspace_bytes,
+                                        _p(out), out_row_stride))
 
 
 def swiglu(stream, n, gate, up, out):
