@@ -104,7 +104,10 @@ struct AttnRows {
             for (int k = 0; k < KS; k++) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) x[k][j] = __fmul_rn(__fmul_rn(__fmul_rn(x[k][j], up), up2), 4.0f * c);
-                split_hi_lo8(x[k], qa[mt][k], ql[mt][k]);
+                // (not split_hi_lo8: of a product the compiler takes hi twice, rounded from
+                // the product for the operand and from its f32 for lo, which near a tie of
+                // the two leaves lo an fp16 step off: 1e-4 of such a row, one row in 250)
+                split_hi_lo8_mix(x[k], qa[mt][k], ql[mt][k]);
             }
             f[mt] = __fmul_rn(pow2_int(e), 0.25f / 128.0f);
             m[mt] = -3.402823466e38f;

@@ -221,6 +221,27 @@ def test_decode_fp8_scales_far_apart(rf, stream):
     check(run_decode(rf, stream, c, q, nh, nkv, hd, seq), want, A, seq, vmax)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_q_next_to_a_tie_of_its_first_term(rf, stream, hd):
+    """q whose product with the softmax factor rounds to another fp16 value
+    than the product rounded to f32 does: its two terms must belong together.
+    K is a multiple of the identity, so each score shows one element of q, and
+    one step of its first term off (2^-11) is 60 times the bound and more."""
+    rng = np.random.default_rng(hd)
+    f = np.float64(np.float32(4) * (np.float32(1.4426950408889634) * (np.float32(1) / np.sqrt(np.float32(hd)))))
+    x = rng.uniform(1, 2, 8000000).astype(np.float32)
+    x = x[(x * f).astype(np.float16) != (x * f).astype(np.float32).astype(np.float16)]
+    batch = min(len(x), 32) // 2
+    assert batch >= 8
+    q = np.stack([np.roll(np.resize(x, hd), b) for b in range(2 * batch)]).reshape(batch, 2, hd).astype(np.float32)
+    c = Cache(rf, stream, rng, HEAD, 1, hd, hd, hd, True)
+    k, ks = kv8.encode(32 * np.eye(hd, dtype=np.float32)[:, None])
+    c.val[0] = kv8.decode(k, ks)
+    c.dev[:2] = [_dev(rf, lay(k, HEAD), stream), _dev(rf, ks.T, stream)]
+    want, A, vmax = prefix_want(c, None, q, 1, hd, None)
+    check(run_prefix(rf, stream, c, None, q, 2, 1, hd, hd, 0, None), want, A, hd, vmax)
+
+
 # ------------------------------------------------------------------ causal rows
 def run_prefill(rf, stream, c, q, nh, nkv, hd, pos0, rows):
     rs = nh * hd + 4
