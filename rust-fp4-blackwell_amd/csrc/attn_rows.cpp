@@ -58,7 +58,7 @@ int check_rows(const char *what, const float *q, uint32_t q_rs, const float *out
 // How a call is cut: the kernel by its query rows of a KV head, the keys into
 // splits.
 struct Plan {
-    int mt, wk;
+    const char *kernel;
     uint32_t tiles0, splits0, chunk0, splits1, chunk1;
     uint32_t splits() const { return splits0 + splits1; }
 };
@@ -76,18 +76,12 @@ void cut(uint64_t keys, uint64_t others, uint64_t least, uint32_t *splits, uint3
     *splits = (uint32_t)((keys + c - 1) / c);
 }
 
-Plan plan(uint32_t nkv, uint32_t group, uint32_t rows, uint64_t len0, uint64_t cap1)
+Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t rows, uint64_t len0, uint64_t cap1)
 {
     Plan p{};
     const uint64_t flat = (uint64_t)rows * group;
-    if (flat <= 16) {
-        p.mt = 1;
-        p.wk = 4;
-    } else {
-        p.mt = 2;
-        p.wk = 1;
-    }
-    const uint64_t rw = 16u * (uint64_t)p.mt * (4u / (uint64_t)p.wk);
+    const uint64_t rw = flat <= 32 ? 16 : flat <= 64 ? 64 : 128;
+    p.kernel = rw == 16 ? "few" : rw == 64 ? (causal ? "causal1" : "many1") : causal ? "causal2" : "many2";
     if (len0) {
         p.tiles0 = (uint32_t)((flat + rw - 1) / rw);
         cut(len0, (uint64_t)p.tiles0 * nkv, 256, &p.splits0, &p.chunk0);
@@ -121,7 +115,7 @@ int run(const char *what, const Plan &p, AttnRowsArgs &a, bool fp8, uint32_t hd,
         return set_error(RFP4_E_CAPACITY, "%s: %llu workgroups (at most 2^23)", what, (unsigned long long)std::max(items, merges));
     char name[64];
     if (items) {
-        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_t%dk%d", hd, fp8 ? "fp8" : "f16", p.mt, p.wk);
+        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_%s", hd, fp8 ? "fp8" : "f16", p.kernel);
         if (int rc = launch(name, dim3((unsigned)items), dim3(256), s, &a)) return rc;
     }
     if (p.splits() == 1) return RFP4_OK;
@@ -179,7 +173,7 @@ int causal(const char *what, hipStream_t s, uint32_t nh, uint32_t nkv, uint32_t 
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = rows; a.causal = 1; a.pos0 = pos0; a.len0 = (uint32_t)keys;
-    return run(what, plan(nkv, nh / nkv, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
+    return run(what, plan(true, nkv, nh / nkv, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
 }
 
 int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint32_t nh, uint32_t nkv, uint32_t hd, const float *q, uint32_t q_rs,
@@ -207,7 +201,7 @@ int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint3
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = batch; a.len0 = prefix; a.cap1 = max_suffix;
-    return run(what, plan(nkv, nh / nkv, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
+    return run(what, plan(false, nkv, nh / nkv, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
 }
 
 } // namespace
@@ -233,7 +227,7 @@ int kv_append_rows_fp8(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads,
 size_t attn_prefill_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows)
 {
     if (check_heads("attn_prefill_fp8_workspace", n_heads, n_kv_heads, head_dim) || rows == 0) return 0;
-    return plan_bytes(plan(n_kv_heads, n_heads / n_kv_heads, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
+    return plan_bytes(plan(true, n_kv_heads, n_heads / n_kv_heads, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
 }
 
 size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq)
@@ -244,7 +238,7 @@ size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t
 size_t attn_decode_prefix_workspace(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t prefix, uint32_t max_suffix)
 {
     if (check_heads("attn_decode_prefix_workspace", n_heads, n_kv_heads, head_dim) || batch == 0) return 0;
-    return plan_bytes(plan(n_kv_heads, n_heads / n_kv_heads, batch, prefix, max_suffix), batch, n_heads, head_dim);
+    return plan_bytes(plan(false, n_kv_heads, n_heads / n_kv_heads, batch, prefix, max_suffix), batch, n_heads, head_dim);
 }
 
 int attn_decode_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq, const float *q,

@@ -51,24 +51,23 @@ struct AttnRowsKeys {
     uint32_t end;           // keys that exist, at least hi
 };
 
-template <int HD, bool F8, int MT, int WK>
-struct AttnRows {
-    static constexpr int KS = HD / 32;          // K steps of S
-    static constexpr int NN = HD / 16;          // dimension tiles of O
-    static constexpr int EB = F8 ? 1 : 2;       // bytes of an element
-    static constexpr int NKL = HD * EB / 64;    // 16-byte K loads of a lane per 16-key half
-    static constexpr int VW = NN * EB / 4;      // dwords of a lane per V row
-    static constexpr int ROWS = 16 * MT * (4 / WK); // query rows of a workgroup
+// A wave's MT tiles of 16 query rows: lane (q4, l16) works for row l16 of each.
+template <int HD, int MT>
+struct AttnRowsState {
+    static constexpr int KS = HD / 32; // K steps of S
+    static constexpr int NN = HD / 16; // dimension tiles of O
 
     uint32_t l16, q4, lane;
-    int wave, kgrp;
     f16x8 qa[MT][KS], ql[MT][KS];
     f32x4 o[MT][NN];
     float m[MT], l[MT], f[MT]; // running maximum and sum, the scores' factor less 2^kref
     uint32_t lim[MT];          // keys that the lane's row sees
 
     // q of the lane's row of each tile, scaled by a power of two of its own to
-    // at most 256, and that scale's inverse into the scores' factor
+    // at most 256, and that scale's inverse into the scores' factor.  PAIRED:
+    // the dimensions of K step k in this lane as 16-byte loads of 8-bit K rows
+    // hold them, two steps a load
+    template <bool PAIRED>
     RFP4_DEV void load_q(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, uint32_t row_end, uint32_t limit0)
     {
         // log2(e) / sqrt(HD) in two factors: the score's factor a power of two,
@@ -86,8 +85,7 @@ struct AttnRows {
             float amax = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                // the dimensions of K step k in this lane: an 8-bit load of 16 covers two steps
-                const uint32_t d = F8 ? 64u * (uint32_t)(k / 2) + 16u * q4 + 8u * (uint32_t)(k % 2) : 32u * (uint32_t)k + 8u * q4;
+                const uint32_t d = PAIRED ? 64u * (uint32_t)(k / 2) + 16u * q4 + 8u * (uint32_t)(k % 2) : 32u * (uint32_t)k + 8u * q4;
                 const float4 x0 = *(const float4 *)(qp + d), x1 = *(const float4 *)(qp + d + 4);
                 x[k][0] = x0.x; x[k][1] = x0.y; x[k][2] = x0.z; x[k][3] = x0.w;
                 x[k][4] = x1.x; x[k][5] = x1.y; x[k][6] = x1.z; x[k][7] = x1.w;
@@ -116,6 +114,90 @@ struct AttnRows {
             for (int n = 0; n < NN; n++) o[mt][n] = {0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
+
+    // The scores of tile mt over the 32 keys from key0 (st: S^T of the two
+    // 16-key halves, the lane's keys 4 q4 .. +3 of each; nan: the keys of scale
+    // byte 255) to probabilities as two fp16 terms; keys at and past `hi` are
+    // masked.  fk: the scores' factor.
+    template <bool F8>
+    RFP4_DEV void probabilities(int mt, const f32x4 (&st)[2], uint32_t key0, uint32_t hi, uint32_t nan, float fk, f16x8 &ph, f16x8 &pl)
+    {
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = st[j / 4][j % 4];
+        // (the empty asm keeps what these rare branches compute out of the loop's registers)
+        if (F8 && nan) {
+            uint32_t k0 = 4u * q4;
+            asm volatile("" : "+v"(k0));
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if ((nan >> (k0 + (uint32_t)(j < 4 ? j : 12 + j))) & 1u) p[j] = __uint_as_float(0x7FC00000u);
+        }
+        // masked scores at -infinity (p = 0 whatever maximum is subtracted)
+        const uint32_t last = min(lim[mt], hi);
+        if (__any(key0 + 32u > last)) {
+            uint32_t k0 = key0 + 4u * q4;
+            asm volatile("" : "+v"(k0));
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k0 + (uint32_t)(j < 4 ? j : 12 + j) >= last) p[j] = -INFINITY;
+        }
+        // online softmax in base 2; the subtracted maximum is raised only when
+        // a score of the row exceeds it by more than 8 (p at most 2^8), so the
+        // common block has no cross-lane step
+        float mx = p[0];
+#pragma unroll
+        for (int j = 1; j < 8; j++) mx = fmaxf(mx, p[j]);
+        mx *= fk;
+        if (__any(mx > m[mt] + 8.0f)) {
+            const float top = xor32_max(xor16_max(mx));
+            const float mnew = top > m[mt] + 8.0f ? top : m[mt];
+            const float alpha = __builtin_amdgcn_exp2f(m[mt] - mnew);
+            m[mt] = mnew;
+            l[mt] *= alpha;
+#pragma unroll
+            for (int n = 0; n < NN; n++) o[mt][n] *= alpha;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], fk, -m[mt]));
+            l[mt] += p[j];
+        }
+        split_hi_lo8_mix(p, ph, pl);
+    }
+
+    // f * 2^(kref - 127), never 0 or infinite: a masked score times it stays -infinity
+    RFP4_DEV float factor(int mt, int kref) const
+    {
+        return fminf(fmaxf(ldexpf(f[mt], kref - 127), 1.17549435e-38f), 3.402823466e38f);
+    }
+    RFP4_DEV void scale_o(float by)
+    {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int n = 0; n < NN; n++) o[mt][n] *= by;
+    }
+};
+
+// Key groups whose K and V go to the registers.
+template <int HD, bool F8, int MT, int WK>
+struct AttnRows : AttnRowsState<HD, MT> {
+    typedef AttnRowsState<HD, MT> State;
+    using State::KS;
+    using State::NN;
+    using State::l16;
+    using State::q4;
+    using State::lane;
+    using State::qa;
+    using State::ql;
+    using State::o;
+    using State::f;
+    static constexpr int EB = F8 ? 1 : 2;       // bytes of an element
+    static constexpr int NKL = HD * EB / 64;    // 16-byte K loads of a lane per 16-key half
+    static constexpr int VW = NN * EB / 4;      // dwords of a lane per V row
+    static constexpr int ROWS = 16 * MT * (4 / WK); // query rows of a workgroup
+    int wave, kgrp;
 
     uint4 kr[2][NKL];    // raw K rows l16 and 16 + l16 of a block
     uint32_t vr[8][VW];  // raw V of the lane's 8 keys
@@ -203,16 +285,11 @@ struct AttnRows {
                     if (kt > kref + 7) {
                         kref = kt;
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) // never 0 or infinite: a masked score times it stays -infinity
-                            fk[mt] = fminf(fmaxf(ldexpf(f[mt], kref - 127), 1.17549435e-38f), 3.402823466e38f);
+                        for (int mt = 0; mt < MT; mt++) fk[mt] = this->factor(mt, kref);
                     }
                     if (vt > vref + 7) {
-                        const float down = pow2_int(vref - vt); // 2^-126 for the first block, whose O is 0
+                        this->scale_o(pow2_int(vref - vt)); // 2^-126 for the first block, whose O is 0
                         vref = vt;
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                            for (int n = 0; n < NN; n++) o[mt][n] *= down;
                     }
                 }
                 sc[lane] = bad ? 1.0f : pow2_int((int)sb - (lane < 32u ? kref : vref));
@@ -246,47 +323,7 @@ struct AttnRows {
             if (more) load_k(s, next);
             f16x8 ph[MT], pl[MT];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float p[8];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) p[4 * h + r] = st[mt][h][r];
-                if (F8 && nan) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if ((nan >> (4u * q4 + (uint32_t)(j < 4 ? j : 12 + j))) & 1u) p[j] = __uint_as_float(0x7FC00000u);
-                }
-                // masked scores at -infinity (p = 0 whatever maximum is subtracted)
-                if (__any(key0 + 32u > min(lim[mt], s.hi))) {
-                    const uint32_t last = min(lim[mt], s.hi);
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (key0 + 4u * q4 + (uint32_t)(j < 4 ? j : 12 + j) >= last) p[j] = -INFINITY;
-                }
-                // online softmax in base 2; the subtracted maximum is raised
-                // only when a score of the row exceeds it by more than 8 (p at
-                // most 2^8), so the common block has no cross-lane step
-                float mx = p[0];
-#pragma unroll
-                for (int j = 1; j < 8; j++) mx = fmaxf(mx, p[j]);
-                mx *= fk[mt];
-                if (__any(mx > m[mt] + 8.0f)) {
-                    const float top = xor32_max(xor16_max(mx));
-                    const float mnew = top > m[mt] + 8.0f ? top : m[mt];
-                    const float alpha = __builtin_amdgcn_exp2f(m[mt] - mnew);
-                    m[mt] = mnew;
-                    l[mt] *= alpha;
-#pragma unroll
-                    for (int n = 0; n < NN; n++) o[mt][n] *= alpha;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], fk[mt], -m[mt]));
-                    l[mt] += p[j];
-                }
-                split_hi_lo8_mix(p, ph[mt], pl[mt]);
-            }
+            for (int mt = 0; mt < MT; mt++) this->template probabilities<F8>(mt, st[mt], key0, s.hi, nan, fk[mt], ph[mt], pl[mt]);
             // ---- O^T += V^T P^T, dimension tiles NB at a time
             constexpr int NB = F8 ? 4 : 2; // tiles of a V dword
 #pragma unroll
@@ -309,11 +346,7 @@ struct AttnRows {
             key0 = next;
         }
         if constexpr (F8) {
-            const float up = ldexpf(1.0f, vref - 127);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int n = 0; n < NN; n++) o[mt][n] *= up;
+            this->scale_o(ldexpf(1.0f, vref - 127));
         }
     }
 
@@ -365,113 +398,308 @@ struct AttnRows {
     }
 };
 
-// One (rows, keys) item of a workgroup: the query rows row0 .. row_end of KV
-// head kvh over s, written as outputs, or as split `split`'s states.
-template <int HD, bool F8, int MT, int WK>
-RFP4_DEV void attn_rows_item(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, uint32_t row_end, const AttnRowsKeys &s,
-                             uint32_t limit0, uint32_t split)
+// Query rows enough for 4 waves of MT tiles each: all of them take every key,
+// which the workgroup stages in LDS as fp16 rows, block by block, two stages:
+// while a block's scores and P V are computed from one, the next block goes
+// from registers (loaded a block earlier) through the conversion into the
+// other, so a key is converted once for 64 MT rows.  V^T operands come out of
+// the rows through the transposing LDS read.  Rows are padded (K by 16 bytes:
+// read 16 rows at a time, 16 bytes each; V by 32: 8 rows, 32 bytes), so reads
+// cover the banks once and every address is one register and a constant.
+// Dimension 16 n + 4 q4 + r is accumulator r of tile n.
+template <int HD, bool F8, int MT>
+struct AttnRowsTile : AttnRowsState<HD, MT> {
+    typedef AttnRowsState<HD, MT> State;
+    using State::KS;
+    using State::NN;
+    using State::l16;
+    using State::q4;
+    using State::lane;
+    using State::qa;
+    using State::ql;
+    using State::o;
+    static constexpr uint32_t EB = F8 ? 1 : 2;
+    static constexpr uint32_t BK = 4096 / HD;   // keys of a block: 32 of 128 dimensions, 64 of 64
+    static constexpr uint32_t KRB = 2 * HD + 16, VRB = 2 * HD + 32; // bytes of a staged K and V row
+    static constexpr uint32_t NL = EB;          // 16-byte loads of a thread for a block's K (and V)
+    static constexpr uint32_t CPR = HD * EB / 16; // 16-byte pieces of a cache row
+    static constexpr uint32_t VOFF = BK * KRB, STAGE = VOFF + BK * VRB; // a block's K rows, then its V rows
+    typedef short i16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+    uint4 kraw[NL], vraw[NL];
+    uint32_t kb, vb;        // scale bytes of key lane % BK of the block in the registers
+    int kref = -1000, vref = -1000;
+    uint64_t nan = 0;       // its keys of byte 255
+
+    // Piece i of thread t: row and 16-byte piece of a block's K or V
+    RFP4_DEV static uint32_t piece_row(uint32_t t, uint32_t i) { return (t + 256u * i) / CPR; }
+    RFP4_DEV static uint32_t piece_col(uint32_t t, uint32_t i) { return (t + 256u * i) % CPR; }
+
+    RFP4_DEV void load(const AttnRowsKeys &s, uint32_t key0)
+    {
+        if (s.ts < (1ull << 24) && key0 + BK <= s.end) { // 32-bit lane offsets from uniform bases
+            const uint8_t *k = s.k + (uint64_t)key0 * s.ts * EB, *v = s.v + (uint64_t)key0 * s.ts * EB;
+#pragma unroll
+            for (uint32_t i = 0; i < NL; i++) {
+                const uint32_t off = piece_row(threadIdx.x, i) * (uint32_t)s.ts * EB + 16u * piece_col(threadIdx.x, i);
+                kraw[i] = *(const uint4 *)(k + off);
+                vraw[i] = *(const uint4 *)(v + off);
+            }
+            if constexpr (F8) {
+                const uint64_t t = (uint64_t)key0 * (s.ts / HD);
+                const uint32_t off = lane % BK * (uint32_t)(s.ts / HD);
+                kb = (s.ks + t)[off];
+                vb = (s.vs + t)[off];
+            }
+        } else { // keys past the last that exists re-read it; they are masked
+            uint32_t tid = threadIdx.x;
+            asm volatile("" : "+v"(tid)); // nothing of this path is held over the loop
+#pragma unroll
+            for (uint32_t i = 0; i < NL; i++) {
+                const uint64_t off = (uint64_t)min(key0 + piece_row(tid, i), s.end - 1u) * s.ts * EB + 16u * piece_col(tid, i);
+                kraw[i] = *(const uint4 *)(s.k + off);
+                vraw[i] = *(const uint4 *)(s.v + off);
+            }
+            if constexpr (F8) {
+                const uint64_t t = (uint64_t)min(key0 + tid % BK, s.end - 1u) * (s.ts / HD);
+                kb = s.ks[t];
+                vb = s.vs[t];
+            }
+        }
+    }
+
+    // The block in the registers as fp16 rows of the stage at st; moves the
+    // references (the same in every wave: all hold the same bytes)
+    RFP4_DEV void stage(lds_u8 *st)
+    {
+        if constexpr (F8) {
+            const bool bad = kb == 255u || vb == 255u;
+            nan = __ballot(bad);
+            if (__any(!bad && ((int)kb > kref + 7 || (int)vb > vref + 7))) {
+                const int kt = __builtin_amdgcn_readfirstlane((int)wave_max(bad ? -2000.0f : (float)kb)); // exact in f32
+                const int vt = __builtin_amdgcn_readfirstlane((int)wave_max(bad ? -2000.0f : (float)vb));
+                kref = kt > kref + 7 ? kt : kref;
+                vref = vt > vref + 7 ? vt : vref;
+            }
+            const uint32_t r = piece_row(threadIdx.x, 0), c = piece_col(threadIdx.x, 0);
+            const float ks = __shfl(bad ? 1.0f : pow2_int((int)kb - kref), (int)r, 64), vs = __shfl(bad ? 1.0f : pow2_int((int)vb - vref), (int)r, 64);
+            uint4 w[2];
+            widen(kraw[0], ks, w);
+            put(st + r * KRB + 32u * c, w[0]);
+            put(st + r * KRB + 32u * c + 16u, w[1]);
+            widen(vraw[0], vs, w);
+            put(st + VOFF + r * VRB + 32u * c, w[0]);
+            put(st + VOFF + r * VRB + 32u * c + 16u, w[1]);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < NL; i++) {
+                const uint32_t r = piece_row(threadIdx.x, i), c = piece_col(threadIdx.x, i);
+                put(st + r * KRB + 16u * c, kraw[i]);
+                put(st + VOFF + r * VRB + 16u * c, vraw[i]);
+            }
+        }
+    }
+    RFP4_DEV static void put(lds_u8 *p, uint4 v) { *(__attribute__((address_space(3))) uint4 *)p = v; }
+    RFP4_DEV static void widen(uint4 r, float scale, uint4 (&w)[2])
+    {
+        const uint32_t x[4] = {r.x, r.y, r.z, r.w};
+        uint32_t y[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, false));
+            y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i], scale, true));
+        }
+        w[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        w[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+
+    // Keys s.lo .. s.hi of the workgroup, of which this wave's rows see those below whi
+    RFP4_DEV void walk(const AttnRowsKeys &s, uint32_t whi, lds_u8 *lds)
+    {
+        // the transposing read: lane j of 16 gives the address of 4 halves, row
+        // j / 4 of 4, columns 4 (j % 4) .. +3 of 16, and gets column j of the 4 rows
+        const uint32_t kaddr = l16 * KRB + 16u * q4, vaddr = VOFF + (4u * q4 + (l16 >> 2)) * VRB + 8u * (l16 & 3u);
+        load(s, s.lo);
+        stage(lds);
+        float fk[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) fk[mt] = F8 ? this->factor(mt, kref) : this->f[mt];
+        int kcur = kref, vcur = vref; // the references of the block that is computed
+        uint64_t nan_now = nan;
+        uint32_t buf = 0;
+        if (s.lo + BK < s.hi) load(s, s.lo + BK);
+        __syncthreads();
+        for (uint32_t key0 = s.lo;; key0 += BK) {
+            if constexpr (F8) {
+                if (kref != kcur || vref != vcur) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) fk[mt] = this->factor(mt, kref);
+                    this->scale_o(pow2_int(vcur - vref));
+                    kcur = kref;
+                    vcur = vref;
+                }
+                nan_now = nan;
+            }
+            const bool more = s.hi - key0 > BK;
+            if (more) {
+                stage(lds + (buf ^ 1u) * STAGE);
+                if (s.hi - key0 > 2u * BK) load(s, key0 + 2u * BK);
+            }
+            lds_u8 *st = lds + buf * STAGE;
+#pragma unroll
+            for (uint32_t c = 0; c < BK / 32u; c++) {
+                if (key0 + 32u * c >= whi) break; // the same for the whole wave
+                f32x4 sc[MT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) sc[mt][0] = sc[mt][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    f16x8 ka[2];
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; h++)
+                        ka[h] = *(const __attribute__((address_space(3))) f16x8 *)(st + kaddr + 64u * (uint32_t)k + (32u * c + 16u * h) * KRB);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) sc[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[h], qa[mt][k], sc[mt][h], 0, 0, 0);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) sc[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[h], ql[mt][k], sc[mt][h], 0, 0, 0);
+                }
+                f16x8 ph[MT], pl[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+                    this->template probabilities<F8>(mt, sc[mt], key0 + 32u * c, s.hi, (uint32_t)(nan_now >> (32u * c)), fk[mt], ph[mt], pl[mt]);
+#pragma unroll
+                for (int n = 0; n < NN; n++) {
+                    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(st + vaddr + 32u * (uint32_t)n + 32u * c * VRB));
+                    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(st + vaddr + 32u * (uint32_t)n + (32u * c + 16u) * VRB));
+                    typedef short i16x8 __attribute__((ext_vector_type(8)));
+                    const f16x8 va = __builtin_bit_cast(f16x8, i16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) o[mt][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[mt], o[mt][n], 0, 0, 0);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) o[mt][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[mt], o[mt][n], 0, 0, 0);
+                }
+            }
+            if (!more) break;
+            __syncthreads();
+            buf ^= 1u;
+        }
+        if constexpr (F8) this->scale_o(ldexpf(1.0f, vcur - 127));
+    }
+};
+
+// Dimensions d .. d + 3 of (row i, head): the output, or of a split's state
+// (first: with the row's maximum and sum)
+template <int HD>
+RFP4_DEV void attn_rows_put(const AttnRowsArgs &a, uint32_t i, uint32_t head, uint32_t S, uint32_t split, uint32_t d, bool first, float M, float L,
+                            f32x4 acc)
 {
+    if (S > 1u) {
+        float *dst = a.part + ((size_t)((size_t)i * a.n_heads + head) * S + split) * (HD + 4);
+        if (first) {
+            dst[0] = M;
+            dst[1] = L;
+        }
+        *(f32x4 *)(dst + 4 + d) = acc;
+    } else { // no key: 0, not 0 / 0; a NaN sum stays NaN
+        const bool none = L == 0.0f;
+        f32x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : __fdiv_rn(acc[j], L);
+        *(f32x4 *)(a.out + (size_t)i * a.out_rs + (size_t)head * HD + d) = y;
+    }
+}
+
+// One item of a workgroup with few rows: the query rows row0 .. row_end (at
+// most 16 MT) of KV head kvh over s by 4 key groups, written as outputs, or as
+// split `split`'s states.
+template <int HD, bool F8, int MT>
+RFP4_DEV void attn_rows_few(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, uint32_t row_end, const AttnRowsKeys &s, uint32_t split)
+{
+    constexpr int WK = 4;
     typedef AttnRows<HD, F8, MT, WK> R;
-    __shared__ __align__(16) float sc[4][64];
+    __shared__ __align__(16) float sc[WK][64];
     R r;
     r.lane = threadIdx.x & 63u;
     r.l16 = r.lane & 15u;
     r.q4 = r.lane >> 4;
-    r.wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    r.kgrp = r.wave % WK;
-    const uint32_t wrow = row0 + 16u * MT * (uint32_t)(r.wave / WK);
-    if (WK == 1 && wrow >= row_end) return; // no barrier with one key group
-    r.load_q(a, kvh, wrow, row_end, limit0);
-    uint32_t whi = s.hi;
-    if (a.causal) whi = min(whi, a.pos0 + min(wrow + 16u * MT - 1u, row_end - 1u) / a.group + 1u);
-    if (wrow < row_end) r.walk(s, whi, sc[r.wave]);
+    r.kgrp = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    r.template load_q<F8>(a, kvh, row0, row_end, s.hi);
+    r.walk(s, s.hi, sc[r.kgrp]);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) r.l[mt] = xor32_sum(xor16_sum(r.l[mt]));
     const uint32_t S = a.splits0 + a.splits1;
 
-    if constexpr (WK == 1) {
+    // the key groups' states through LDS
+    constexpr int RW = 16 * MT, LD = HD + 4;
+    __shared__ __align__(16) float ro[WK][RW][LD];
+    __shared__ float rm[WK][RW], rl[WK][RW];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            const uint32_t rho = wrow + 16u * (uint32_t)mt + r.l16;
-            if (rho >= row_end) continue;
-            const uint32_t i = rho / a.group, head = kvh * a.group + rho % a.group;
-            float *dst;
-            float inv = 1.0f;
-            if (S > 1u) {
-                dst = a.part + ((size_t)((size_t)i * a.n_heads + head) * S + split) * (HD + 4) + 4;
-                if (r.q4 == 0u) {
-                    dst[-4] = r.m[mt];
-                    dst[-3] = r.l[mt];
-                }
-            } else {
-                dst = a.out + (size_t)i * a.out_rs + (size_t)head * HD;
-                inv = r.l[mt];
-            }
-            // (no key: 0, not 0 / 0; a NaN sum stays NaN)
-            const bool none = inv == 0.0f;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int n = 0; n < R::NN; n += 4) {
-                    float y[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : __fdiv_rn(r.o[mt][n + j][t], inv);
-                    *(float4 *)(dst + (4u * r.q4 + (uint32_t)t) * R::NN + n) = make_float4(y[0], y[1], y[2], y[3]);
-                }
+    for (int mt = 0; mt < MT; mt++) {
+        const uint32_t row = 16u * (uint32_t)mt + r.l16;
+        if (r.q4 == 0u) {
+            rm[r.kgrp][row] = r.m[mt];
+            rl[r.kgrp][row] = r.l[mt];
         }
-    } else {
-        // the key groups' states through LDS
-        constexpr int RW = R::ROWS, LD = HD + 4;
-        __shared__ __align__(16) float ro[WK][RW][LD];
-        __shared__ float rm[WK][RW], rl[WK][RW];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            const uint32_t row = 16u * (uint32_t)(MT * (r.wave / WK) + mt) + r.l16;
-            if (r.q4 == 0u) {
-                rm[r.kgrp][row] = r.m[mt];
-                rl[r.kgrp][row] = r.l[mt];
-            }
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int n = 0; n < R::NN; n += 4)
+                *(float4 *)&ro[r.kgrp][row][(4u * r.q4 + (uint32_t)t) * R::NN + n] =
+                    make_float4(r.o[mt][n][t], r.o[mt][n + 1][t], r.o[mt][n + 2][t], r.o[mt][n + 3][t]);
+    }
+    __syncthreads();
+    constexpr uint32_t LPR = HD / 4; // lanes of a row, 4 dimensions each
+    for (uint32_t u = threadIdx.x; u < (uint32_t)RW * LPR; u += 256u) {
+        const uint32_t row = u / LPR, d = 4u * (u % LPR), rho = row0 + row;
+        if (rho >= row_end) break;
+        float M = rm[0][row];
 #pragma unroll
-                for (int n = 0; n < R::NN; n += 4)
-                    *(float4 *)&ro[r.kgrp][row][(4u * r.q4 + (uint32_t)t) * R::NN + n] =
-                        make_float4(r.o[mt][n][t], r.o[mt][n + 1][t], r.o[mt][n + 2][t], r.o[mt][n + 3][t]);
+        for (int g = 1; g < WK; g++) M = fmaxf(M, rm[g][row]);
+        float L = 0.0f;
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int g = 0; g < WK; g++) {
+            const float w = __builtin_amdgcn_exp2f(rm[g][row] - M);
+            L = fmaf(rl[g][row], w, L);
+            const f32x4 x = *(const f32x4 *)&ro[g][row][d];
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j] = fmaf(x[j], w, acc[j]);
         }
-        __syncthreads();
-        constexpr uint32_t LPR = HD / 4; // lanes of a row, 4 dimensions each
-        for (uint32_t u = threadIdx.x; u < (uint32_t)RW * LPR; u += 256u) {
-            const uint32_t row = u / LPR, d = 4u * (u % LPR), rho = row0 + row;
-            if (rho >= row_end) break;
-            float M = rm[0][row];
+        attn_rows_put<HD>(a, rho / a.group, kvh * a.group + rho % a.group, S, split, d, d == 0u, M, L, acc);
+    }
+}
+
+// The same for up to 64 MT rows, whose waves take all keys each.
+template <int HD, bool F8, int MT>
+RFP4_DEV void attn_rows_many(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, uint32_t row_end, const AttnRowsKeys &s, uint32_t split)
+{
+    typedef AttnRowsTile<HD, F8, MT> R;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * R::STAGE];
+    R r;
+    r.lane = threadIdx.x & 63u;
+    r.l16 = r.lane & 15u;
+    r.q4 = r.lane >> 4;
+    const uint32_t wrow = row0 + 16u * MT * (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    r.template load_q<false>(a, kvh, wrow, row_end, s.hi);
+    uint32_t whi = wrow < row_end ? s.hi : 0u; // waves without rows stage and wait only
+    if (a.causal) whi = min(whi, a.pos0 + min(wrow + 16u * MT - 1u, row_end - 1u) / a.group + 1u);
+    r.walk(s, whi, (typename R::lds_u8 *)lds);
+    const uint32_t S = a.splits0 + a.splits1;
 #pragma unroll
-            for (int g = 1; g < WK; g++) M = fmaxf(M, rm[g][row]);
-            float L = 0.0f;
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int mt = 0; mt < MT; mt++) {
+        const float L = xor32_sum(xor16_sum(r.l[mt]));
+        const uint32_t rho = wrow + 16u * (uint32_t)mt + r.l16;
+        if (rho >= row_end) continue;
 #pragma unroll
-            for (int g = 0; g < WK; g++) {
-                const float w = __builtin_amdgcn_exp2f(rm[g][row] - M);
-                L = fmaf(rl[g][row], w, L);
-                const f32x4 x = *(const f32x4 *)&ro[g][row][d];
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[j] = fmaf(x[j], w, acc[j]);
-            }
-            const uint32_t i = rho / a.group, head = kvh * a.group + rho % a.group;
-            if (S > 1u) {
-                float *dst = a.part + ((size_t)((size_t)i * a.n_heads + head) * S + split) * (HD + 4);
-                if (d == 0u) {
-                    dst[0] = M;
-                    dst[1] = L;
-                }
-                *(f32x4 *)(dst + 4 + d) = acc;
-            } else {
-                const bool none = L == 0.0f;
-                f32x4 y;
-#pragma unroll
-                for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : __fdiv_rn(acc[j], L);
-                *(f32x4 *)(a.out + (size_t)i * a.out_rs + (size_t)head * HD + d) = y;
-            }
-        }
+        for (int n = 0; n < R::NN; n++)
+            attn_rows_put<HD>(a, rho / a.group, kvh * a.group + rho % a.group, S, split, 16u * (uint32_t)n + 4u * r.q4, n == 0 && r.q4 == 0u, r.m[mt], L,
+                              r.o[mt][n]);
     }
 }
 
@@ -479,43 +707,54 @@ RFP4_DEV void attn_rows_item(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0,
 // XCD, workgroup id % 8, keeps one head's K and V in its L2): the shared keys'
 // items (row tile, split) first, the longest causal ranges leading, then the
 // own keys' (row, split).
-template <int HD, bool F8, int MT, int WK>
+template <int HD, bool F8, int MT, bool MANY, bool OWN>
 RFP4_DEV void attn_rows_body(const AttnRowsArgs &a)
 {
     constexpr uint32_t EB = F8 ? 1u : 2u;
-    constexpr uint32_t RW = 16u * MT * (4 / WK);
+    constexpr uint32_t RW = MANY ? 64u * MT : 16u * MT;
     const uint32_t kvh = blockIdx.x % a.n_kv_heads, item = blockIdx.x / a.n_kv_heads;
-    const uint32_t flat = a.rows * a.group;
+    uint32_t row0, row_end, split;
+    const void *k, *v;
+    const uint8_t *ks, *vs;
+    uint64_t base;
     AttnRowsKeys s;
-    if (item < a.tiles0 * a.splits0) {
-        const uint32_t tile = a.tiles0 - 1u - item / a.splits0, split = item % a.splits0;
-        const uint32_t row0 = tile * RW, row_end = flat;
+    const bool own = OWN && item >= a.tiles0 * a.splits0;
+    if (!own) {
+        const uint32_t tile = a.tiles0 - 1u - item / a.splits0;
+        split = item % a.splits0;
+        row0 = tile * RW;
+        row_end = min(row0 + RW, a.rows * a.group);
         s.lo = split * a.chunk0;
         s.end = a.len0;
         s.hi = min(s.lo + a.chunk0, a.len0);
-        if (a.causal) s.hi = min(s.hi, a.pos0 + (min(row0 + RW, flat) - 1u) / a.group + 1u);
+        if (a.causal) s.hi = min(s.hi, a.pos0 + (row_end - 1u) / a.group + 1u);
         if (s.lo >= s.hi) return;
         s.ts = a.ts0;
-        s.k = (const uint8_t *)a.k0 + (uint64_t)kvh * a.hs0 * EB;
-        s.v = (const uint8_t *)a.v0 + (uint64_t)kvh * a.hs0 * EB;
-        s.ks = F8 ? a.ks0 + (uint64_t)kvh * (a.hs0 / HD) : nullptr;
-        s.vs = F8 ? a.vs0 + (uint64_t)kvh * (a.hs0 / HD) : nullptr;
-        attn_rows_item<HD, F8, MT, WK>(a, kvh, row0, row_end, s, s.hi, split);
+        base = (uint64_t)kvh * a.hs0;
+        k = a.k0; v = a.v0; ks = a.ks0; vs = a.vs0;
     } else {
-        const uint32_t own = item - a.tiles0 * a.splits0, row = own / a.splits1, split = own % a.splits1;
-        const uint32_t len = (uint32_t)__builtin_amdgcn_readfirstlane((int)min(a.lens[row], a.cap1));
-        s.lo = split * a.chunk1;
-        s.end = len;
-        s.hi = min(s.lo + a.chunk1, len);
+        const uint32_t x = item - a.tiles0 * a.splits0, row = x / a.splits1, part = x % a.splits1;
+        s.end = (uint32_t)__builtin_amdgcn_readfirstlane((int)min(a.lens[row], a.cap1));
+        split = a.splits0 + part;
+        row0 = row * a.group;
+        row_end = row0 + a.group;
+        s.lo = part * a.chunk1;
+        s.hi = min(s.lo + a.chunk1, s.end);
         // a split past the row's last key is not merged; with one split in all, the row is 0
-        if (s.lo >= len && a.splits0 + a.splits1 > 1u) return;
-        const uint64_t base = (uint64_t)row * a.ss1 + (uint64_t)kvh * a.hs1;
+        if (s.lo >= s.end && a.splits0 + a.splits1 > 1u) return;
         s.ts = a.ts1;
-        s.k = (const uint8_t *)a.k1 + base * EB;
-        s.v = (const uint8_t *)a.v1 + base * EB;
-        s.ks = F8 ? a.ks1 + base / HD : nullptr;
-        s.vs = F8 ? a.vs1 + base / HD : nullptr;
-        attn_rows_item<HD, F8, 1, 4>(a, kvh, row * a.group, (row + 1u) * a.group, s, s.hi, a.splits0 + split);
+        base = (uint64_t)row * a.ss1 + (uint64_t)kvh * a.hs1;
+        k = a.k1; v = a.v1; ks = a.ks1; vs = a.vs1;
+    }
+    s.k = (const uint8_t *)k + base * EB;
+    s.v = (const uint8_t *)v + base * EB;
+    s.ks = F8 ? ks + base / HD : nullptr;
+    s.vs = F8 ? vs + base / HD : nullptr;
+    if constexpr (MANY) {
+        if (!own) attn_rows_many<HD, F8, MT>(a, kvh, row0, row_end, s, split);
+        else attn_rows_few<HD, F8, 1>(a, kvh, row0, row_end, s, split);
+    } else {
+        attn_rows_few<HD, F8, MT>(a, kvh, row0, row_end, s, split);
     }
 }
 
