@@ -316,6 +316,11 @@ int mx4_quantize_tiled(rfp4_stream_t stream, uint64_t rows, uint64_t k, const vo
 int fp4_gemm_tiled(rfp4_stream_t stream, uint32_t m, uint32_t n, uint32_t k, const uint8_t *a_codes,
                    const uint8_t *a_scales, const uint8_t *a_scales_tiled, const uint8_t *w_codes,
                    const uint8_t *w_scales, const uint8_t *w_scales_tiled, float *c);
+/* Test hook (this thread): the kernel of later attn_decode_fp8,
+ * attn_prefill_fp8 and attn_decode_prefix_* calls (and their _workspace
+ * functions): 0 = planned, 1 = 16 query rows for a workgroup, 2 = 64.  No
+ * reference counterpart. */
+int rfp4_debug_attn_rows(int mode);
 /* Test hook: force the GEMM tile (index into the compiled list, largest
  * first: 256x256, 256x128, 128x128, 64x128, 32x128, then 5 = the few-row
  * kernel for k a multiple of 512, up to 16384 for m <= 32 and up to 8192

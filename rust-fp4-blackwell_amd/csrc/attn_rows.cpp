@@ -55,38 +55,62 @@ int check_rows(const char *what, const float *q, uint32_t q_rs, const float *out
     return RFP4_OK;
 }
 
+thread_local int t_mode = 0; // 0 planned, 1 attn_rows_few, 2 attn_rows_many
+
 // How a call is cut: the kernel by its query rows of a KV head, the keys into
 // splits.
 struct Plan {
-    const char *kernel;
+    bool many;
     uint32_t tiles0, splits0, chunk0, splits1, chunk1;
     uint32_t splits() const { return splits0 + splits1; }
 };
 
-// Workgroups that fill the chip: two of 4 waves on each of its 256 CUs.
-constexpr uint64_t kWorkgroups = 512;
-
-void cut(uint64_t keys, uint64_t others, uint64_t least, uint32_t *splits, uint32_t *chunk)
+// Splits of keys for `others` workgroups that the other dimensions give: n, in
+// chunks of 128 (what a workgroup takes in a step).
+void cut(uint64_t keys, uint64_t n, uint32_t *splits, uint32_t *chunk)
 {
-    // as many splits as the other dimensions leave workgroups for, of at least `least` keys, whole blocks of 4 waves
-    uint64_t n = std::max<uint64_t>(1, kWorkgroups / std::max<uint64_t>(1, others));
-    n = std::max<uint64_t>(1, std::min(n, keys / least));
+    n = std::max<uint64_t>(1, n);
     const uint64_t c = ((keys + n - 1) / n + 127) / 128 * 128;
     *chunk = (uint32_t)c;
     *splits = (uint32_t)((keys + c - 1) / c);
 }
 
-Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t rows, uint64_t len0, uint64_t cap1)
+Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t hd, uint32_t rows, uint64_t len0, uint64_t cap1)
 {
     Plan p{};
     const uint64_t flat = (uint64_t)rows * group;
-    const uint64_t rw = flat <= 32 ? 16 : flat <= 64 ? 64 : 128;
-    p.kernel = rw == 16 ? "few" : rw == 64 ? (causal ? "causal1" : "many1") : causal ? "causal2" : "many2";
+    // 16 query rows for a workgroup whose waves read keys of their own, or 64 for
+    // one that stages them: the first reads and converts a key for every 16 rows
+    // and starts sooner, so few rows or keys are its.  The line is a number of
+    // scores, query heads x keys.  Measured (us, few / many): heads of 128, 400
+    // prompt rows 17.6 / 18.0 (2.6e6 scores), 512 20.1 / 19.9 (4.2e6), 700 29.7 /
+    // 25.8 (7.8e6), 64 rows over 2048 shared fp16 keys 21.0 / 25.1 (4.2e6), 4096
+    // 29.3 / 25.6 (8.4e6), 16384 83.8 / 48.8; 8 bits, 4096 25.7 / 29.7, 8192 38.4 /
+    // 35.4, 16384 67.9 / 50.9; heads of 64, 700 prompt rows 16.7 / 19.2 (7.8e6),
+    // 1024 24.3 / 23.1 (1.7e7), 64 rows over 4096 fp16 keys 20.2 / 20.1 (8.4e6).  Up
+    // to 32 rows of a KV head the second wastes half its waves (20 rows of 64 over
+    // 4096 keys 10.5 / 13.5).
+    const uint64_t keys = causal ? (uint64_t)rows * (len0 - rows) + (uint64_t)rows * (rows + 1u) / 2u : (uint64_t)rows * len0;
+    p.many = flat > 32 && keys * group * nkv > (hd == 128 ? 6000000u : 12000000u);
+    if (t_mode) p.many = t_mode == 2;
+    const uint64_t rw = p.many ? 64u : 16u;
+    // As many splits as make a workgroup for each of 256 CUs, of at least 128 keys
+    // (a block for each wave; 8 heads x 4096 keys: 128 keys 6.2 us and 2.7 to merge,
+    // 256 7.2 and 2.5), and 256 for the staging kernel (64 rows over 4096 keys: 128
+    // keys 15.8 + 4.0, 256 13.8 + 3.4, 512 25.3 + 4.5); for that two workgroups a CU
+    // where a split keeps 2048 keys (256 rows after 16384 keys 165 -> 141 us; with
+    // 1024 left 64 rows over 16384 50.9 -> 52.8, with 256 over 4096 25.6 -> 31.5).
     if (len0) {
         p.tiles0 = (uint32_t)((flat + rw - 1) / rw);
-        cut(len0, (uint64_t)p.tiles0 * nkv, 256, &p.splits0, &p.chunk0);
+        const uint64_t wgs = (uint64_t)p.tiles0 * nkv;
+        uint64_t n = std::min<uint64_t>(256u / wgs, len0 / (p.many ? 256u : 128u));
+        if (p.many) n = std::max(n, std::min<uint64_t>(512u / wgs, len0 / 2048u));
+        cut(len0, n, &p.splits0, &p.chunk0);
     }
-    if (cap1) cut(cap1, (uint64_t)rows * nkv, 256, &p.splits1, &p.chunk1);
+    // The rows' own keys, a workgroup for each row's query heads: the first kernel's,
+    // in a launch of its own where the second takes the shared ones, unless they are
+    // few (run()).
+    if (cap1) cut(cap1, std::min<uint64_t>(256u / ((uint64_t)rows * nkv), cap1 / 128u), &p.splits1, &p.chunk1);
     return p;
 }
 
@@ -109,13 +133,22 @@ int run(const char *what, const Plan &p, AttnRowsArgs &a, bool fp8, uint32_t hd,
     a.chunk0 = p.chunk0;
     a.splits1 = p.splits1;
     a.chunk1 = p.chunk1;
-    const uint64_t items = ((uint64_t)p.tiles0 * p.splits0 + (uint64_t)a.rows * p.splits1) * a.n_kv_heads;
-    const uint64_t merges = (uint64_t)a.rows * a.n_heads;
-    if (std::max(items, merges) > ((uint64_t)1 << 23))
-        return set_error(RFP4_E_CAPACITY, "%s: %llu workgroups (at most 2^23)", what, (unsigned long long)std::max(items, merges));
+    const uint64_t shared = (uint64_t)p.tiles0 * p.splits0 * a.n_kv_heads, own = (uint64_t)a.rows * p.splits1 * a.n_kv_heads;
+    const uint64_t merges = (uint64_t)a.rows * a.n_heads, most = std::max(shared + own, merges);
+    if (most > ((uint64_t)1 << 22))
+        return set_error(RFP4_E_CAPACITY, "%s: %llu workgroups (at most 2^22)", what, (unsigned long long)most);
     char name[64];
-    if (items) {
-        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_%s", hd, fp8 ? "fp8" : "f16", p.kernel);
+    const char *type = fp8 ? "fp8" : "f16";
+    // few own keys beside the shared ones of the second kernel, in its launch: 64
+    // rows of up to 300 own keys over 16384 shared 51.8 us, in two launches 58.3
+    const uint64_t many = !p.many ? 0u : a.cap1 <= 512u ? shared + own : shared;
+    if (many) {
+        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_many", hd, type);
+        if (int rc = launch(name, dim3((unsigned)many), dim3(512), s, &a)) return rc;
+    }
+    a.first = (uint32_t)(many / a.n_kv_heads);
+    if (const uint64_t items = shared + own - many) {
+        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_few", hd, type);
         if (int rc = launch(name, dim3((unsigned)items), dim3(256), s, &a)) return rc;
     }
     if (p.splits() == 1) return RFP4_OK;
@@ -173,7 +206,7 @@ int causal(const char *what, hipStream_t s, uint32_t nh, uint32_t nkv, uint32_t 
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = rows; a.causal = 1; a.pos0 = pos0; a.len0 = (uint32_t)keys;
-    return run(what, plan(true, nkv, nh / nkv, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
+    return run(what, plan(true, nkv, nh / nkv, hd, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
 }
 
 int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint32_t nh, uint32_t nkv, uint32_t hd, const float *q, uint32_t q_rs,
@@ -201,12 +234,19 @@ int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint3
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = batch; a.len0 = prefix; a.cap1 = max_suffix;
-    return run(what, plan(false, nkv, nh / nkv, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
+    return run(what, plan(false, nkv, nh / nkv, hd, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
 }
 
 } // namespace
 
 extern "C" {
+
+int rfp4_debug_attn_rows(int mode)
+{
+    if (mode < 0 || mode > 2) return set_error(RFP4_E_INVALID, "attention of rows: mode %d (0, 1 or 2)", mode);
+    t_mode = mode;
+    return RFP4_OK;
+}
 
 int kv_append_rows_f16(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, const uint32_t *positions,
                        const float *k, uint32_t k_row_stride, const float *v, uint32_t v_row_stride, uint16_t *kc, uint16_t *vc,
@@ -227,7 +267,7 @@ int kv_append_rows_fp8(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads,
 size_t attn_prefill_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows)
 {
     if (check_heads("attn_prefill_fp8_workspace", n_heads, n_kv_heads, head_dim) || rows == 0) return 0;
-    return plan_bytes(plan(true, n_kv_heads, n_heads / n_kv_heads, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
+    return plan_bytes(plan(true, n_kv_heads, n_heads / n_kv_heads, head_dim, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
 }
 
 size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq)
@@ -238,7 +278,7 @@ size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t
 size_t attn_decode_prefix_workspace(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t prefix, uint32_t max_suffix)
 {
     if (check_heads("attn_decode_prefix_workspace", n_heads, n_kv_heads, head_dim) || batch == 0) return 0;
-    return plan_bytes(plan(false, n_kv_heads, n_heads / n_kv_heads, batch, prefix, max_suffix), batch, n_heads, head_dim);
+    return plan_bytes(plan(false, n_kv_heads, n_heads / n_kv_heads, head_dim, batch, prefix, max_suffix), batch, n_heads, head_dim);
 }
 
 int attn_decode_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq, const float *q,

@@ -179,25 +179,18 @@ K256 void rfp4_attn_merge_hd64(AttnArgs a) { attn_merge_body<64>(a); }
 K256 void rfp4_attn_merge_hd128(AttnArgs a) { attn_merge_body<128>(a); }
 
 // ---- the 8-bit cache, and attention of rows and batches
-// (device/kv_rows.h, device/attn_rows.h): rfp4_attn_rows_hd<HD>_<type>_t<MT>k<WK>,
-// 16 MT (4 / WK) query rows and WK key groups per workgroup (attn_rows.cpp)
+// (device/kv_rows.h, device/attn_rows.h): rfp4_attn_rows_hd<HD>_<type>_few,
+// 16 query rows for a workgroup, and _many, 64 (attn_rows.cpp picks)
 #define K256W2 extern "C" __global__ __launch_bounds__(256, 2)
-#define K256W3 extern "C" __global__ __launch_bounds__(256, 3)
+#define K512W4 extern "C" __global__ __launch_bounds__(512, 4)
 #define ATTN_ROWS_KERNELS(HD, NAME, F8) \
     K256 void rfp4_kv_rows_hd##HD##_##NAME(KvRowsArgs a) { kv_rows_body<HD, F8>(a); } \
-    K256W2 void rfp4_attn_rows_hd##HD##_##NAME##_few(AttnRowsArgs a) { attn_rows_body<HD, F8, 1, false, true>(a); } \
-    K256W2 void rfp4_attn_rows_hd##HD##_##NAME##_many1(AttnRowsArgs a) { attn_rows_body<HD, F8, 1, true, true>(a); } \
-    K256W2 void rfp4_attn_rows_hd##HD##_##NAME##_many2(AttnRowsArgs a) { attn_rows_body<HD, F8, 2, true, true>(a); }
+    K256W2 void rfp4_attn_rows_hd##HD##_##NAME##_few(AttnRowsArgs a) { attn_rows_body<HD, F8, false>(a); } \
+    K512W4 void rfp4_attn_rows_hd##HD##_##NAME##_many(AttnRowsArgs a) { attn_rows_body<HD, F8, true>(a); }
 ATTN_ROWS_KERNELS(64, fp8, true)
 ATTN_ROWS_KERNELS(64, f16, false)
 ATTN_ROWS_KERNELS(128, fp8, true)
 ATTN_ROWS_KERNELS(128, f16, false)
-// no keys of a row's own: prompt rows
-#define ATTN_CAUSAL_KERNELS(HD) \
-    K256W3 void rfp4_attn_rows_hd##HD##_fp8_causal1(AttnRowsArgs a) { attn_rows_body<HD, true, 1, true, false>(a); } \
-    K256W2 void rfp4_attn_rows_hd##HD##_fp8_causal2(AttnRowsArgs a) { attn_rows_body<HD, true, 2, true, false>(a); }
-ATTN_CAUSAL_KERNELS(64)
-ATTN_CAUSAL_KERNELS(128)
 K256 void rfp4_attn_rows_merge_hd64(AttnRowsArgs a) { attn_rows_merge_body<64>(a); }
 K256 void rfp4_attn_rows_merge_hd128(AttnRowsArgs a) { attn_rows_merge_body<128>(a); }
 

@@ -160,6 +160,7 @@ typedef struct KvRowsArgs {
 // Attention of query rows over a cache of 8 bits or fp16 (device/attn_rows.h).
 // Keys: `0` those that every row may see (len0 of them; causal: row i the
 // first pos0 + i + 1), `1` each row's own, the first min(lens[i], cap1).
+enum { kAttnRowsMaxSplits = 1024 }; // splits0 + splits1: what the merge kernel holds
 typedef struct AttnRowsArgs {
     const float *q;            // row i: q + i*q_rs, [n_heads][head_dim]
     float *out;                // row i: out + i*out_rs
@@ -172,6 +173,7 @@ typedef struct AttnRowsArgs {
     uint32_t causal, pos0, len0, cap1;
     uint32_t tiles0, splits0, chunk0;       // row tiles and key splits of `0`
     uint32_t splits1, chunk1;               // key splits of each row of `1`
+    uint32_t first;                         // item of workgroup 0
 } AttnRowsArgs;
 
 // Batched prefill row kernels (device/prefill.h).

@@ -118,6 +118,7 @@ _SIGS = {
     "mx4_quantize_tiled": (I32, [P, U64, U64, P, I32, P, P, P]),
     "rfp4_debug_gemm_plan": (I32, [I32, I32]),
     "rfp4_debug_attn_chunk": (I32, [U32]),
+    "rfp4_debug_attn_rows": (I32, [I32]),
     "rfp4_gemm_plan": (I32, [U32, U32, U32, P, P, P]),
     "rfp4_gemm_plan_kernel": (I32, [U32, U32, U32, C.c_char_p, SZ]),
     "rfp4_prefill_epilogue_kernel": (I32, [U32, U32, U32, U32, C.c_char_p, SZ]),

@@ -11,6 +11,15 @@ from test_gpu_kernels import _dev
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=[1, 2], ids=["few", "many"])
+def kernel(rf, request):
+    """Both kernels of the attention calls at every size (the planner gives the second large ones only)."""
+    rf.check(rf.load().rfp4_debug_attn_rows(request.param))
+    yield request.param
+    rf.check(rf.load().rfp4_debug_attn_rows(0))
+
+
 HEAD, TOKEN = "head", "token"
 
 
@@ -174,7 +183,7 @@ def attend_head(c, q, kvh, keys):
 
 @pytest.mark.parametrize("seq", [1, 2, 31, 32, 33, 96, 127, 128, 129, 255, 256, 257, 511, 513, 1000, 4097, 20000])
 @pytest.mark.parametrize("nh,nkv,hd,layout", [(8, 2, 128, HEAD), (8, 1, 64, TOKEN), (3, 3, 128, TOKEN), (10, 2, 64, HEAD), (32, 8, 128, HEAD)])
-def test_decode_fp8(rf, stream, nh, nkv, hd, layout, seq):
+def test_decode_fp8(rf, stream, kernel, nh, nkv, hd, layout, seq):
     if seq > 5000 and nh > 8:
         seq = 5003
     rng = np.random.default_rng(seq + nh)
@@ -186,7 +195,7 @@ def test_decode_fp8(rf, stream, nh, nkv, hd, layout, seq):
 
 @pytest.mark.parametrize("mag", [1e-30, 1e-12, 1e-4, 1e3, 1e15, 1e30])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_decode_fp8_magnitudes(rf, stream, hd, mag):
+def test_decode_fp8_magnitudes(rf, stream, kernel, hd, mag):
     """q and K of any size whose products are ordinary scores, and tiny q over a cache with rows of zeros."""
     nh, nkv, seq = 4, 2, 301
     rng = np.random.default_rng(hd)
@@ -200,7 +209,7 @@ def test_decode_fp8_magnitudes(rf, stream, hd, mag):
     check(run_decode(rf, stream, z, q * np.float32(1e-8 if mag < 1 else 1), nh, nkv, hd, seq), want, A, seq, vmax)
 
 
-def test_decode_fp8_scales_far_apart(rf, stream):
+def test_decode_fp8_scales_far_apart(rf, stream, kernel):
     """Rows whose scales spread over 2^-20 .. 2^20 in any order: rows far below
     the largest still count where the large ones get no weight.  A K row is off
     by at most 2^-41 of the largest K (2^-34 of the reference's scale), a V row
@@ -222,7 +231,7 @@ def test_decode_fp8_scales_far_apart(rf, stream):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
-def test_q_next_to_a_tie_of_its_first_term(rf, stream, hd):
+def test_q_next_to_a_tie_of_its_first_term(rf, stream, kernel, hd):
     """q whose product with the softmax factor rounds to another fp16 value
     than the product rounded to f32 does: its two terms must belong together.
     K is a multiple of the identity, so each score shows one element of q, and
@@ -272,7 +281,7 @@ def prefill_want(c, q, group, pos0):
 
 @pytest.mark.parametrize("pos0,rows", [(0, 1), (0, 2), (0, 16), (0, 17), (0, 33), (0, 130), (31, 1), (33, 5), (95, 33), (250, 70), (4000, 3), (3001, 64), (0, 515)])
 @pytest.mark.parametrize("nh,nkv,hd,layout", [(8, 2, 128, HEAD), (8, 1, 64, TOKEN), (3, 3, 64, HEAD), (6, 2, 128, TOKEN), (7, 1, 128, HEAD)])
-def test_prefill_fp8(rf, stream, nh, nkv, hd, layout, pos0, rows):
+def test_prefill_fp8(rf, stream, kernel, nh, nkv, hd, layout, pos0, rows):
     rng = np.random.default_rng(pos0 * 31 + rows + nh)
     c = Cache(rf, stream, rng, layout, nkv, pos0 + rows, pos0 + rows + 37, hd, True)
     q = rng.standard_normal((rows, nh, hd)).astype(np.float32)
@@ -282,7 +291,7 @@ def test_prefill_fp8(rf, stream, nh, nkv, hd, layout, pos0, rows):
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("which", [1, 3])
-def test_prefill_fp8_nan_rows(rf, stream, hd, which):
+def test_prefill_fp8_nan_rows(rf, stream, kernel, hd, which):
     """A K or V row with scale byte 255 at position t: every row from t on is NaN, the rows before it are as if it were not there."""
     nh, nkv, pos0, rows, t = 4, 1, 20, 100, 77
     rng = np.random.default_rng(hd + which)
@@ -297,7 +306,7 @@ def test_prefill_fp8_nan_rows(rf, stream, hd, which):
     assert np.isnan(got[t - pos0:]).all()
 
 
-def test_prefill_fp8_growing_scores(rf, stream):
+def test_prefill_fp8_growing_scores(rf, stream, kernel):
     """Scores tens apart, so that most blocks raise a row's maximum."""
     nh, nkv, hd, pos0, rows = 4, 1, 128, 40, 150
     rng = np.random.default_rng(5)
@@ -308,7 +317,7 @@ def test_prefill_fp8_growing_scores(rf, stream):
 
 
 @pytest.mark.parametrize("rows", [1, 40])
-def test_offsets_past_32_bits(rf, stream, rows):
+def test_offsets_past_32_bits(rf, stream, kernel, rows):
     """A token stride of 2^24 elements and more: the last of 301 tokens lies past 5 GB."""
     nh, nkv, hd, seq, ts = 4, 2, 64, 301, (1 << 24) + 64
     rng = np.random.default_rng(rows)
@@ -360,7 +369,7 @@ def prefix_want(p, s, q, nkv, prefix, lens):
 @pytest.mark.parametrize("fp8", [True, False])
 @pytest.mark.parametrize("batch,prefix,cap", [(1, 0, 1), (1, 1, 0), (1, 300, 5), (2, 0, 40), (3, 33, 0), (3, 517, 33), (5, 1000, 130), (9, 64, 700), (17, 257, 1), (40, 129, 9)])
 @pytest.mark.parametrize("nh,nkv,hd,layout", [(8, 2, 128, HEAD), (8, 1, 64, TOKEN), (3, 3, 64, HEAD), (10, 2, 128, TOKEN)])
-def test_prefix(rf, stream, fp8, nh, nkv, hd, layout, batch, prefix, cap):
+def test_prefix(rf, stream, kernel, fp8, nh, nkv, hd, layout, batch, prefix, cap):
     rng = np.random.default_rng(batch * 7 + prefix + cap + nh)
     p = Cache(rf, stream, rng, layout, nkv, prefix, prefix + 3, hd, fp8) if prefix else None
     s = Cache(rf, stream, rng, layout, nkv, cap, cap, hd, fp8, lead=(batch,)) if cap else None
@@ -375,7 +384,7 @@ def test_prefix(rf, stream, fp8, nh, nkv, hd, layout, batch, prefix, cap):
 
 
 @pytest.mark.parametrize("fp8", [True, False])
-def test_prefix_empty_rows_and_long_lengths(rf, stream, fp8):
+def test_prefix_empty_rows_and_long_lengths(rf, stream, kernel, fp8):
     """Rows without any token are 0; a length past max_suffix counts as max_suffix; what lies behind a row's last token is not read as a value."""
     nh, nkv, hd, cap = 4, 2, 64, 300
     rng = np.random.default_rng(1)
@@ -462,6 +471,19 @@ def test_prompt_tokens_then_a_batch(rf, stream):
         check(out.to_host(3 * nh * hd, np.float32, stream).reshape(3, nh, hd), want, A, seen + 4, vmax)
 
 
+@pytest.mark.parametrize("fp8,nh,nkv,hd,batch,prefix", [(True, 8, 2, 128, 33, 24500), (False, 8, 1, 64, 40, 40000)])
+@pytest.mark.parametrize("cap", [65, 700])
+def test_planned_for_many_rows(rf, stream, fp8, nh, nkv, hd, batch, prefix, cap):
+    """Sizes on the far side of the planner's line, with own keys in the same launch and in one of their own."""
+    rng = np.random.default_rng(batch)
+    p = Cache(rf, stream, rng, TOKEN, nkv, prefix, prefix, hd, fp8)
+    s = Cache(rf, stream, rng, HEAD, nkv, cap, cap, hd, fp8, lead=(batch,))
+    lens = rng.integers(0, cap + 1, batch).astype(np.uint32)
+    q = rng.standard_normal((batch, nh, hd)).astype(np.float32)
+    want, A, vmax = prefix_want(p, s, q, nkv, prefix, lens)
+    check(run_prefix(rf, stream, p, s, q, nh, nkv, hd, prefix, cap, lens), want, A, prefix + cap, vmax)
+
+
 def test_prefix_over_an_engines_cache(rf, stream):
     """The shared cache is an engine's; against attn_decode_f16 on the same memory."""
     cfg = rf.model_config(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=1024, theta=10000.0, eps=1e-5, max_seq=300)
@@ -486,7 +508,7 @@ def test_prefix_over_an_engines_cache(rf, stream):
 
 
 # ------------------------------------------------------------------ streams and graphs
-def test_two_streams_at_once(rf, stream):
+def test_two_streams_at_once(rf, stream, kernel):
     """Calls that overlap, each with its own workspace, give what each gives alone."""
     nh, nkv, hd, seq = 8, 2, 128, 6000
     rng = np.random.default_rng(4)
@@ -506,7 +528,7 @@ def test_two_streams_at_once(rf, stream):
         np.testing.assert_array_equal(out[i].to_host(nh * hd, np.float32, stream).reshape(nh, hd), alone[i])
 
 
-def test_captured_and_replayed(rf):
+def test_captured_and_replayed(rf, kernel):
     """An append and a batch step in a graph, replayed with new rows, positions
     and lengths in the same buffers, each replay against the calls themselves."""
     hip = C.CDLL("libamdhip64.so")

@@ -117,6 +117,10 @@ def test_workspace_sizes():
     assert rfp4.attn_decode_prefix_workspace(4, 32, 8, 128, 100, 100) >= 2 * 4 * 32 * 132 * 4
 
 
+def test_the_kernel_hook():
+    assert [rfp4.load().rfp4_debug_attn_rows(m) for m in (-1, 3, 2, 1, 0)] == [-1, -1, 0, 0, 0]
+
+
 def test_the_oracle_format():
     """The tests' encoder: levels encode to themselves, ties go to the even code, scales as defined."""
     codes, scales = kv8.encode(np.concatenate((kv8.LEVELS, -kv8.LEVELS))[None].astype(np.float32))
