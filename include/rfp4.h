@@ -192,9 +192,11 @@ int attn_prefill_f16(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads
  *
  * These calls share nothing: each works in the caller's workspace (16-byte
  * aligned, of any content, at least the bytes that the call's _workspace
- * function says for the same arguments; 0 bytes may be NULL), so calls on
- * several streams need a workspace each, and so do captured graphs that may
- * run at once.  They only launch kernels and may be captured. */
+ * function says; 0 bytes may be NULL; the size for a context (seq, pos0,
+ * prefix, max_suffix) is enough for every shorter one, for other rows, heads
+ * or batches it is another), so calls on several streams need a workspace
+ * each, and so do captured graphs that may run at once.  They only launch
+ * kernels and may be captured. */
 /* New rows of K and V (f32; row r at k + r*k_row_stride, v + r*v_row_stride,
  * [n_kv_heads][head_dim]) into a cache, fp16 (RNE) or 8 bits: for each row and
  * KV head the smallest scale 2^e, e >= -127, with which the largest magnitude

@@ -5,7 +5,6 @@
 #include "runtime.h"
 
 #include <algorithm>
-#include <cstdio>
 
 using namespace rfp4;
 
@@ -65,15 +64,34 @@ struct Plan {
     uint32_t splits() const { return splits0 + splits1; }
 };
 
-// Splits of keys for `others` workgroups that the other dimensions give: n, in
-// chunks of 128 (what a workgroup takes in a step).
+// n splits or fewer, in chunks of a multiple of 128 keys (a workgroup's step).
 void cut(uint64_t keys, uint64_t n, uint32_t *splits, uint32_t *chunk)
 {
-    n = std::max<uint64_t>(1, n);
     const uint64_t c = ((keys + n - 1) / n + 127) / 128 * 128;
     *chunk = (uint32_t)c;
     *splits = (uint32_t)((keys + c - 1) / c);
 }
+
+// Splits of `keys` shared keys at most, for `tiles` row tiles: as many as make a
+// workgroup for each of 256 CUs, of at least 128 keys (a block for each wave; 8
+// heads x 4096 keys: 128 keys 6.2 us and 2.7 to merge, 256 7.2 and 2.5), and 256
+// for the staging kernel (64 rows over 4096 keys: 128 keys 15.8 + 4.0, 256 13.8 +
+// 3.4, 512 25.3 + 4.5); for that two workgroups a CU where a split keeps 2048 keys
+// (256 rows after 16384 keys 165 -> 141 us; with 1024 left 64 rows over 16384 50.9
+// -> 52.8, with 256 over 4096 25.6 -> 31.5).  Never fewer for more keys; 512 and
+// 256 of the rows' own at most, within the merge's kAttnRowsMaxSplits.
+uint64_t splits_of(bool many, uint64_t keys, uint64_t tiles, uint32_t nkv)
+{
+    const uint64_t wgs = tiles * nkv;
+    uint64_t n = std::min<uint64_t>(256u / wgs, keys / (many ? 256u : 128u));
+    if (many) n = std::max(n, std::min<uint64_t>(512u / wgs, keys / 2048u));
+    return std::max<uint64_t>(1, n);
+}
+uint64_t splits_of_own(uint64_t keys, uint32_t rows, uint32_t nkv)
+{
+    return std::max<uint64_t>(1, std::min<uint64_t>(256u / ((uint64_t)rows * nkv), keys / 128u));
+}
+uint64_t tiles_of(bool many, uint64_t flat) { return many ? (flat + 63) / 64 : (flat + 15) / 16; }
 
 Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t hd, uint32_t rows, uint64_t len0, uint64_t cap1)
 {
@@ -93,35 +111,38 @@ Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t hd, uint32_t rows,
     const uint64_t keys = causal ? (uint64_t)rows * (len0 - rows) + (uint64_t)rows * (rows + 1u) / 2u : (uint64_t)rows * len0;
     p.many = flat > 32 && keys * group * nkv > (hd == 128 ? 6000000u : 12000000u);
     if (t_mode) p.many = t_mode == 2;
-    const uint64_t rw = p.many ? 64u : 16u;
-    // As many splits as make a workgroup for each of 256 CUs, of at least 128 keys
-    // (a block for each wave; 8 heads x 4096 keys: 128 keys 6.2 us and 2.7 to merge,
-    // 256 7.2 and 2.5), and 256 for the staging kernel (64 rows over 4096 keys: 128
-    // keys 15.8 + 4.0, 256 13.8 + 3.4, 512 25.3 + 4.5); for that two workgroups a CU
-    // where a split keeps 2048 keys (256 rows after 16384 keys 165 -> 141 us; with
-    // 1024 left 64 rows over 16384 50.9 -> 52.8, with 256 over 4096 25.6 -> 31.5).
     if (len0) {
-        p.tiles0 = (uint32_t)((flat + rw - 1) / rw);
-        const uint64_t wgs = (uint64_t)p.tiles0 * nkv;
-        uint64_t n = std::min<uint64_t>(256u / wgs, len0 / (p.many ? 256u : 128u));
-        if (p.many) n = std::max(n, std::min<uint64_t>(512u / wgs, len0 / 2048u));
-        cut(len0, n, &p.splits0, &p.chunk0);
+        p.tiles0 = (uint32_t)tiles_of(p.many, flat);
+        cut(len0, splits_of(p.many, len0, p.tiles0, nkv), &p.splits0, &p.chunk0);
     }
     // The rows' own keys, a workgroup for each row's query heads: the first kernel's,
     // in a launch of its own where the second takes the shared ones, unless they are
     // few (run()).
-    if (cap1) cut(cap1, std::min<uint64_t>(256u / ((uint64_t)rows * nkv), cap1 / 128u), &p.splits1, &p.chunk1);
+    if (cap1) cut(cap1, splits_of_own(cap1, rows, nkv), &p.splits1, &p.chunk1);
     return p;
 }
 
-size_t plan_bytes(const Plan &p, uint32_t rows, uint32_t nh, uint32_t hd)
+size_t state_bytes(uint64_t splits, uint32_t rows, uint32_t nh, uint32_t hd)
 {
-    return p.splits() > 1 ? (size_t)rows * nh * p.splits() * (hd + 4) * sizeof(float) : 0;
+    return splits > 1 ? (size_t)rows * nh * splits * (hd + 4) * sizeof(float) : 0;
+}
+
+// A workspace for the split states of up to len0 shared and cap1 own keys: a chunk
+// is a whole number of steps, so fewer keys can take more splits.
+size_t workspace_bytes_of(uint32_t nkv, uint32_t nh, uint32_t hd, uint32_t rows, uint64_t len0, uint64_t cap1)
+{
+    const uint64_t flat = (uint64_t)rows * (nh / nkv);
+    const bool either = flat > 32 && !t_mode, many = t_mode == 2;
+    uint64_t n = 0;
+    if (len0) n = splits_of(many, len0, tiles_of(many, flat), nkv);
+    if (len0 && either) n = std::max(n, splits_of(true, len0, tiles_of(true, flat), nkv));
+    if (cap1) n += splits_of_own(cap1, rows, nkv);
+    return state_bytes(n, rows, nh, hd);
 }
 
 int run(const char *what, const Plan &p, AttnRowsArgs &a, bool fp8, uint32_t hd, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
-    const size_t need = plan_bytes(p, a.rows, a.n_heads, hd);
+    const size_t need = state_bytes(p.splits(), a.rows, a.n_heads, hd);
     if (need && !workspace) return set_error(RFP4_E_INVALID, "%s: null workspace (%zu bytes)", what, need);
     if (need && !aligned(workspace, 16)) return set_error(RFP4_E_ALIGN, "%s: workspace must be 16-byte aligned", what);
     if (need > workspace_bytes)
@@ -137,19 +158,19 @@ int run(const char *what, const Plan &p, AttnRowsArgs &a, bool fp8, uint32_t hd,
     const uint64_t merges = (uint64_t)a.rows * a.n_heads, most = std::max(shared + own, merges);
     if (most > ((uint64_t)1 << 22))
         return set_error(RFP4_E_CAPACITY, "%s: %llu workgroups (at most 2^22)", what, (unsigned long long)most);
-    char name[64];
-    const char *type = fp8 ? "fp8" : "f16";
+    static const char *const kNames[2][2][2] = { // [head dim 128][8 bits][many]
+        {{"rfp4_attn_rows_hd64_f16_few", "rfp4_attn_rows_hd64_f16_many"}, {"rfp4_attn_rows_hd64_fp8_few", "rfp4_attn_rows_hd64_fp8_many"}},
+        {{"rfp4_attn_rows_hd128_f16_few", "rfp4_attn_rows_hd128_f16_many"}, {"rfp4_attn_rows_hd128_fp8_few", "rfp4_attn_rows_hd128_fp8_many"}}};
+    const char *const *const names = kNames[hd == 128][fp8];
     // few own keys beside the shared ones of the second kernel, in its launch: 64
     // rows of up to 300 own keys over 16384 shared 51.8 us, in two launches 58.3
     const uint64_t many = !p.many ? 0u : a.cap1 <= 512u ? shared + own : shared;
     if (many) {
-        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_many", hd, type);
-        if (int rc = launch(name, dim3((unsigned)many), dim3(512), s, &a)) return rc;
+        if (int rc = launch(names[1], dim3((unsigned)many), dim3(512), s, &a)) return rc;
     }
     a.first = (uint32_t)(many / a.n_kv_heads);
     if (const uint64_t items = shared + own - many) {
-        snprintf(name, sizeof name, "rfp4_attn_rows_hd%u_%s_few", hd, type);
-        if (int rc = launch(name, dim3((unsigned)items), dim3(256), s, &a)) return rc;
+        if (int rc = launch(names[0], dim3((unsigned)items), dim3(256), s, &a)) return rc;
     }
     if (p.splits() == 1) return RFP4_OK;
     // the splits' states, or the zeros of rows that have no keys at all
@@ -185,9 +206,8 @@ int append_rows(const char *what, bool fp8, hipStream_t s, uint32_t rows, uint32
     const uint64_t units = (uint64_t)rows * 2u * nkv, per = 256u / (hd / 8u);
     if (units > ((uint64_t)1 << 27)) return set_error(RFP4_E_CAPACITY, "%s: %u rows of %u heads in one call", what, rows, nkv);
     KvRowsArgs a{k, v, kc, vc, ks, vs, positions, positions ? ss : 0, ts, hs, k_rs, v_rs, rows, nkv, pos0, capacity};
-    char name[48];
-    snprintf(name, sizeof name, "rfp4_kv_rows_hd%u_%s", hd, fp8 ? "fp8" : "f16");
-    return launch(name, dim3((unsigned)((units + per - 1) / per)), dim3(256), s, &a);
+    static const char *const kNames[2][2] = {{"rfp4_kv_rows_hd64_f16", "rfp4_kv_rows_hd64_fp8"}, {"rfp4_kv_rows_hd128_f16", "rfp4_kv_rows_hd128_fp8"}};
+    return launch(kNames[hd == 128][fp8], dim3((unsigned)((units + per - 1) / per)), dim3(256), s, &a);
 }
 
 int causal(const char *what, hipStream_t s, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t pos0, uint32_t rows, const float *q, uint32_t q_rs,
@@ -267,7 +287,7 @@ int kv_append_rows_fp8(rfp4_stream_t stream, uint32_t rows, uint32_t n_kv_heads,
 size_t attn_prefill_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t pos0, uint32_t rows)
 {
     if (check_heads("attn_prefill_fp8_workspace", n_heads, n_kv_heads, head_dim) || rows == 0) return 0;
-    return plan_bytes(plan(true, n_kv_heads, n_heads / n_kv_heads, head_dim, rows, (uint64_t)pos0 + rows, 0), rows, n_heads, head_dim);
+    return workspace_bytes_of(n_kv_heads, n_heads, head_dim, rows, (uint64_t)pos0 + rows, 0);
 }
 
 size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq)
@@ -278,7 +298,7 @@ size_t attn_decode_fp8_workspace(uint32_t n_heads, uint32_t n_kv_heads, uint32_t
 size_t attn_decode_prefix_workspace(uint32_t batch, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t prefix, uint32_t max_suffix)
 {
     if (check_heads("attn_decode_prefix_workspace", n_heads, n_kv_heads, head_dim) || batch == 0) return 0;
-    return plan_bytes(plan(false, n_kv_heads, n_heads / n_kv_heads, head_dim, batch, prefix, max_suffix), batch, n_heads, head_dim);
+    return workspace_bytes_of(n_kv_heads, n_heads, head_dim, batch, prefix, max_suffix);
 }
 
 int attn_decode_fp8(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t seq, const float *q,

@@ -117,6 +117,26 @@ def test_workspace_sizes():
     assert rfp4.attn_decode_prefix_workspace(4, 32, 8, 128, 100, 100) >= 2 * 4 * 32 * 132 * 4
 
 
+@pytest.mark.parametrize("nh,nkv,rows", [(32, 8, 1), (8, 1, 1), (8, 1, 5), (32, 8, 40), (3, 3, 130), (4, 4, 33)])
+def test_a_workspace_serves_every_shorter_context(nh, nkv, rows):
+    lens = sorted({1, 2, 127, 128, 129, 255, 256, 1000, 4095, 4096, 4097, 8191, 12000, 16384, 16500, 33000, 70000, 300000})
+    decode = [rfp4.attn_decode_fp8_workspace(nh, nkv, 128, n) for n in lens]
+    prefill = [rfp4.attn_prefill_fp8_workspace(nh, nkv, 64, n, rows) for n in lens]
+    prefix = [rfp4.attn_decode_prefix_workspace(rows, nh, nkv, 128, n, 700) for n in lens]
+    suffix = [rfp4.attn_decode_prefix_workspace(rows, nh, nkv, 128, 5000, n) for n in lens]
+    for size in (decode, prefill, prefix, suffix):
+        assert size == sorted(size)
+    # and the calls ask for no more than that
+    for n in lens:
+        ws = rfp4.attn_decode_fp8_workspace(nh, nkv, 64, max(lens))
+        assert call("attn_decode_fp8", DECODE, nh=nh, nkv=nkv, seq=n, wsb=ws) == NOT_INIT
+        ws = rfp4.attn_prefill_fp8_workspace(nh, nkv, 128, max(lens), rows)
+        assert call("attn_prefill_fp8", PREFILL, nh=nh, nkv=nkv, pos0=n, rows=rows, wsb=ws, qrs=nh * 128, ors=nh * 128) == NOT_INIT
+        ws = rfp4.attn_decode_prefix_workspace(rows, nh, nkv, 128, max(lens), max(lens))
+        for m in lens:
+            assert call("attn_decode_prefix_fp8", PREFIX, batch=rows, nh=nh, nkv=nkv, prefix=n, cap=m, wsb=ws, qrs=nh * 128, ors=nh * 128) == NOT_INIT
+
+
 def test_the_kernel_hook():
     assert [rfp4.load().rfp4_debug_attn_rows(m) for m in (-1, 3, 2, 1, 0)] == [-1, -1, 0, 0, 0]
 
