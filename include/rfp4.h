@@ -187,8 +187,11 @@ int attn_prefill_f16(rfp4_stream_t stream, uint32_t n_heads, uint32_t n_kv_heads
  * of head_dim) and, in k_scales and v_scales, one E8M0 byte for each row at
  * the row's element offset / head_dim: a value is code * 2^(byte - 127).  Byte
  * 255 makes the whole row NaN; codes 0x7F and 0xFF (NaN) are not used, and
- * what a buffer holds past the tokens that a call names does not matter.  All
- * buffers, and rows of q, k, v and out, 16-byte aligned (scales: any).
+ * what a buffer holds past the tokens that a call names does not matter.  An
+ * infinity or NaN in q, or in an fp16 row, makes the results that it reaches
+ * infinite or NaN; so do 8-bit values so large that 256 times their sum over
+ * the keys leaves f32's range.  All buffers, and rows of q, k, v and out,
+ * 16-byte aligned (scales: any).
  *
  * These calls share nothing: each works in the caller's workspace (16-byte
  * aligned, of any content, at least the bytes that the call's _workspace

@@ -233,7 +233,11 @@ RFP4_DEV void attn_rows_put(const AttnRowsArgs &a, uint32_t i, uint32_t head, ui
 // its operands are through them.
 //
 // Bound by HBM where the keys are many, else by the chain of a launch: loads,
-// scores, softmax, P V, the groups' merge.
+// scores, softmax, P V, the groups' merge.  One row of 32 heads of 128 over 8, 8
+// bits: 32769 keys (68 MB) 15.5-16.4 us, 4.1-4.4 TB/s; 4096 keys 6.2-6.5 us; 77 keys
+// of 4 heads of 64 over one 4.1 us (the whole chain once).  16 rows over 4096 shared
+// fp16 keys read them four times, once for every 4 rows, out of L2: 14.3-15.0 us with
+// their own 200 keys, and from there 1.2 us for every 32 keys of a wave.
 template <int HD, bool F8, int WK>
 struct AttnRowsFew : AttnRowsState<HD> {
     typedef AttnRowsState<HD> State;
@@ -494,8 +498,9 @@ RFP4_DEV void attn_rows_few(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, 
 // other takes exponentials, converts and stages; 4 waves a SIMD (128 registers),
 // two workgroups a CU.  Loads are a step ahead.  What bounds it: both kinds of
 // instruction and their issue; at 2048 rows after 2048 keys of 32 heads of 128
-// over 8 the matrix cores are busy 43 % of the cycles (206 GFLOP with the second
-// terms in 210 us, 0.98 PFLOP/s, where a large fp16 product reaches 1.15).
+// over 8 (206 GFLOP with the second terms) 189-192 us in a row of calls, 1.08
+// PFLOP/s, where a large fp16 product reaches 1.15; under the profiler 210 us, the
+// matrix cores busy 43 % of the cycles.  64 rows over 16384 keys: 50-52 us.
 // Measured there and not better: 32 rows a wave (210 us; free-running 212; with
 // the conversion between the matrix instructions 241), 8 waves of 16 rows and
 // one group (222), 4 groups (259), 32 rows a wave without the rare paths moved
@@ -840,7 +845,8 @@ RFP4_DEV void attn_rows_body(const AttnRowsArgs &a)
 // / sum l 2^(m - M); 0 for a row without keys.  HD / 4 lanes take the dimensions
 // of a state, the workgroup's 1024 / HD parts every so many of the splits; the
 // first four of each part are loaded beside the (m, l) that their weights need,
-// so up to 4096 / HD splits take one round trip of memory.
+// so up to 4096 / HD splits take one round trip of memory: 32 heads of 32 splits
+// 2.6-3.8 us, most of it the launch (9.3 us with a round trip for every 8 of 52).
 template <int HD>
 RFP4_DEV void attn_rows_merge_body(const AttnRowsArgs &a)
 {

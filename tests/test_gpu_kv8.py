@@ -404,6 +404,27 @@ def test_prefix_empty_rows_and_long_lengths(rf, stream, kernel, fp8):
     assert not got.any()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefix_f16_values_that_are_not_finite(rf, stream, kernel, hd):
+    """They reach the rows that read them: an infinite V its dimension, a NaN K the whole row; no other row changes."""
+    nkv, cap = 2, 150
+    rng = np.random.default_rng(hd)
+    p = Cache(rf, stream, rng, HEAD, nkv, 70, 70, hd, False)
+    s = Cache(rf, stream, rng, TOKEN, nkv, cap, cap, hd, False, lead=(5,))
+    lens = np.array([150, 149, 0, 33, 150], np.uint32)
+    q = rng.standard_normal((5, 4, hd)).astype(np.float32)
+    want, A, vmax = prefix_want(p, s, q, nkv, 70, lens)
+    for i, (b, t) in ((0, (4, 149)), (1, (1, 148)), (0, (3, 33)), (1, (3, 40))):  # the last two behind row 3's tokens
+        x = s.val[i].astype(np.float16)
+        x[b, t, 1, 5] = np.nan if i == 0 else np.inf
+        s.val[i] = x.astype(np.float64)
+        s.dev[i] = _dev(rf, lay(x, TOKEN).view(np.uint16), stream)
+    got = run_prefix(rf, stream, p, s, q, 4, nkv, hd, 70, cap, lens)
+    assert np.isnan(got[4, 2:]).all() and not np.isfinite(got[1, 2:, 5]).any()
+    want[4, 2:], want[1, 2:, 5], got[4, 2:], got[1, 2:, 5] = 0, 0, 0, 0
+    check(got, want, A, 70 + cap, vmax)
+
+
 def test_prefix_without_any_keys(rf, stream):
     out = _dev(rf, np.full(3 * 128, 5, np.float32), stream)
     q = _dev(rf, np.ones(3 * 128, np.float32), stream)
