@@ -618,37 +618,43 @@ struct AttnRowsMany : AttnRowsState<HD> {
             u32x4v{fp8x2_to_f16<false>(w0, scale), fp8x2_to_f16<true>(w0, scale), fp8x2_to_f16<false>(w1, scale), fp8x2_to_f16<true>(w1, scale)};
     }
 
-    // S^T of the staged K (kbuf: this lane's address in it)
-    RFP4_DEV void scores(const lds_u8 *kbuf)
+    // O^T += V^T P^T of the staged V (PV), then S^T of the staged K; kbuf and vbuf:
+    // this lane's addresses in them.  An operand of 16 bytes feeds two
+    // instructions, 32 cycles, and takes over 100 from LDS: it is read AHEAD
+    // operands before its use (the scheduling barriers keep that order).
+    template <bool PV>
+    RFP4_DEV void matrix(const lds_u8 *vbuf, const lds_u8 *kbuf)
     {
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                f16x8 ka[2];
-#pragma unroll
-                for (uint32_t h = 0; h < 2; h++)
-                    ka[h] = *(const __attribute__((address_space(3))) f16x8 *)(kbuf + 64u * (uint32_t)k + (32u * (uint32_t)c + 16u * h) * KRB);
-#pragma unroll
-                for (int h = 0; h < 2; h++) sc[c][h] = mfma16(ka[h], qa[k], k ? sc[c][h] : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                for (int h = 0; h < 2; h++) sc[c][h] = mfma16(ka[h], ql[k], sc[c][h]);
-            }
-    }
-    // O^T += V^T P^T of the staged V (vbuf: this lane's address in it)
-    RFP4_DEV void add_pv(const lds_u8 *vbuf)
-    {
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int d = 0; d < NN; d++) {
-                const lds_u8 *const at = vbuf + 32u * (uint32_t)d + 32u * (uint32_t)c * VRB;
+        constexpr int NPV = PV ? NC * NN : 0, N = NPV + NC * KS * 2, AHEAD = 2;
+        f16x8 x[AHEAD + 1];
+        auto fetch = [&](int j) {
+            if (j < NPV) {
+                const lds_u8 *const at = vbuf + 32u * (uint32_t)(j % NN) + 32u * (uint32_t)(j / NN) * VRB;
                 const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)at);
                 const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(at + 16u * VRB));
-                const f16x8 va = __builtin_bit_cast(f16x8, i16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
-                o[d] = mfma16(va, ph[c], o[d]);
-                o[d] = mfma16(va, pl[c], o[d]);
+                return __builtin_bit_cast(f16x8, i16x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
             }
+            const int i = j - NPV, c = i / (2 * KS), k = i / 2 % KS, h = i % 2;
+            return *(const __attribute__((address_space(3))) f16x8 *)(kbuf + 64u * (uint32_t)k + (32u * (uint32_t)c + 16u * (uint32_t)h) * KRB);
+        };
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) x[j] = fetch(j);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            if (j + AHEAD < N) x[(j + AHEAD) % (AHEAD + 1)] = fetch(j + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            const f16x8 y = x[j % (AHEAD + 1)];
+            if (j < NPV) {
+                const int c = j / NN, d = j % NN;
+                o[d] = mfma16(y, ph[c], o[d]);
+                o[d] = mfma16(y, pl[c], o[d]);
+            } else {
+                const int i = j - NPV, c = i / (2 * KS), k = i / 2 % KS, h = i % 2;
+                sc[c][h] = mfma16(y, qa[k], k ? sc[c][h] : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                sc[c][h] = mfma16(y, ql[k], sc[c][h]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 
     RFP4_DEV static void barrier() // with this wave's LDS accesses done; global loads stay in flight
@@ -677,7 +683,7 @@ struct AttnRowsMany : AttnRowsState<HD> {
         load_any(s, s.k, s.ks, key0 + STEP, kraw);
         barrier();
         if (group) barrier(); // half a step behind
-        scores(kl);
+        matrix<false>(vl, kl);
         barrier();
         int kcur = -1001, vcur = -1000; // references of the factor (the first block always sets it) and of O
         // the blocks to load next: V of the next step, K of the one after it
@@ -733,8 +739,7 @@ struct AttnRowsMany : AttnRowsState<HD> {
             // ---- matrix half: P V of the block, the scores of the next
             if (__builtin_expect(live, 1)) {
                 __builtin_amdgcn_s_setprio(1);
-                add_pv(vl);
-                scores(kl);
+                matrix<true>(vl, kl);
                 __builtin_amdgcn_s_setprio(0);
             }
             if (i + 1u == steps) break;
