@@ -496,15 +496,21 @@ RFP4_DEV void attn_rows_few(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, 
 // The groups run half a step apart between common barriers: while one does its
 // matrix instructions (P V of its block, then the scores of its next one), the
 // other takes exponentials, converts and stages; 4 waves a SIMD (128 registers),
-// two workgroups a CU.  Loads are a step ahead.  What bounds it: both kinds of
-// instruction and their issue; at 2048 rows after 2048 keys of 32 heads of 128
-// over 8 (206 GFLOP with the second terms) 189-192 us in a row of calls, 1.08
-// PFLOP/s, where a large fp16 product reaches 1.15; under the profiler 210 us, the
-// matrix cores busy 43 % of the cycles.  64 rows over 16384 keys: 50-52 us.
+// two workgroups a CU.  Loads are a step ahead.  At 2048 rows after 2048 keys of 32
+// heads of 128 over 8 (206 GFLOP with the second terms) 187-195 us in a row of
+// calls, 1.06-1.10 PFLOP/s, where a large fp16 product reaches 1.15; under the
+// profiler 210 us, the matrix cores busy 45 % of the cycles.  64 rows over 16384
+// keys: 51-57 us.  What bounds it there: a vector half takes 1800 cycles, a matrix
+// half 1050 and then waits.  Measured alone on a SIMD, a vector instruction takes
+// 5.4 cycles, an exponential or mixed fma 10, beside matrix instructions 6.7 and 11;
+// the eight loads of a step and their addresses about 550 together.
 // Measured there and not better: 32 rows a wave (210 us; free-running 212; with
 // the conversion between the matrix instructions 241), 8 waves of 16 rows and
 // one group (222), 4 groups (259), 32 rows a wave without the rare paths moved
-// out of the loop's way (305).
+// out of the loop's way (305).  In a row of calls (here 187-198): staging and loads
+// between the matrix instructions, with two buffers (V half 900 cycles, M half 2050:
+// 205), staged rows permuted so that no write meets a bank twice (the same), 16-byte
+// loads and each scale byte loaded once (187).
 template <int HD, bool F8>
 struct AttnRowsMany : AttnRowsState<HD> {
     typedef AttnRowsState<HD> State;
