@@ -493,21 +493,22 @@ RFP4_DEV void attn_rows_few(const AttnRowsArgs &a, uint32_t kvh, uint32_t row0, 
 // 32: 8 rows, 32 bytes), so reads cover the banks once and every address is one
 // register and a constant.  Dimension 16 n + 4 q4 + r is accumulator r of tile n.
 //
-// The groups run half a step apart between common barriers: while one does its
-// matrix instructions (P V of its block, then the scores of its next one), the
+// The groups run half a step apart between common barriers: while one loads and does
+// its matrix instructions (P V of its block, then the scores of its next one), the
 // other takes exponentials, converts and stages; 4 waves a SIMD (128 registers),
-// two workgroups a CU.  Loads are a step ahead.  At 2048 rows after 2048 keys of 32
-// heads of 128 over 8 (206 GFLOP with the second terms) 187-195 us in a row of
-// calls, 1.06-1.10 PFLOP/s, where a large fp16 product reaches 1.15; under the
-// profiler 210 us, the matrix cores busy 45 % of the cycles.  64 rows over 16384
-// keys: 51-57 us.  What bounds it there: a vector half takes 1800 cycles, a matrix
-// half 1050 and then waits.  Measured alone on a SIMD, a vector instruction takes
-// 5.4 cycles, an exponential or mixed fma 10, beside matrix instructions 6.7 and 11;
-// the eight loads of a step and their addresses about 550 together.
+// two workgroups a CU.  At 2048 rows after 2048 keys of 32
+// heads of 128 over 8 (206 GFLOP with the second terms) 186 us in a row of
+// calls, 1.11 PFLOP/s, where a large fp16 product reaches 1.15; under the
+// profiler 207 us, the matrix cores busy 47 % of the cycles.  64 rows over 16384
+// keys: 49-54 us.  What bounds it there: a vector half takes 1500-1650 cycles, a
+// matrix half 1600-1750 with 550 of loads and their addresses (in the vector half
+// those took it to 1800, the whole 188 us), and the waits between 200-450 each.  Alone
+// on a SIMD a wave's vector instruction takes 5.4 cycles, its exponential or mixed
+// fma 9.4, beside another's matrix instructions 6.8 and 11.
 // Measured there and not better: 32 rows a wave (210 us; free-running 212; with
 // the conversion between the matrix instructions 241), 8 waves of 16 rows and
 // one group (222), 4 groups (259), 32 rows a wave without the rare paths moved
-// out of the loop's way (305).  In a row of calls (here 187-198): staging and loads
+// out of the loop's way (305).  In a row of calls (188-198 at the time): staging and loads
 // between the matrix instructions, with two buffers (V half 900 cycles, M half 2050:
 // 205), staged rows permuted so that no write meets a bank twice (the same), 16-byte
 // loads and each scale byte loaded once (187).
@@ -697,7 +698,7 @@ struct AttnRowsMany : AttnRowsState<HD> {
         const uint8_t *vn = s.v + ofs * EB, *kn = s.k + (ofs + step) * EB, *vsn = s.vs + (F8 ? ofs / HD : 0u), *ksn = s.ks + (F8 ? (ofs + step) / HD : 0u);
         const uint32_t in = s.ts < (1ull << 24) ? s.end : 0u; // keys that the 32-bit offsets reach
         for (uint32_t i = 0;; i++, key0 += STEP) {
-            // ---- vector half: the block's probabilities; its V and the next block's K to LDS
+            // ---- vector half: its V and the next block's K to LDS; the block's probabilities
             // (expected branches fall through: a taken one costs the wave a fetch)
             uint64_t nan = 0;
             if constexpr (F8) {
@@ -716,19 +717,6 @@ struct AttnRowsMany : AttnRowsState<HD> {
             }
             stage<VRB>(vbuf, vraw, vref);
             stage<KRB>(kbuf, kraw, kref);
-            if (__builtin_expect(key0 + 2u * STEP + BK <= in, 1)) {
-                load_whole(s, vn, vsn, vraw);
-                load_whole(s, kn, ksn, kraw);
-            } else {
-                load_any(s, s.v, s.vs, key0 + STEP, vraw);
-                load_any(s, s.k, s.ks, key0 + 2u * STEP, kraw);
-            }
-            vn += step * EB;
-            kn += step * EB;
-            if constexpr (F8) {
-                vsn += step / HD;
-                ksn += step / HD;
-            }
             const bool live = key0 < whi; // the same for the whole wave
             if (__builtin_expect(live, 1)) {
                 bool rare = false;
@@ -742,7 +730,20 @@ struct AttnRowsMany : AttnRowsState<HD> {
                 for (int c = 0; c < NC; c++) this->probabilities(sc[c], ph[c], pl[c]);
             }
             barrier();
-            // ---- matrix half: P V of the block, the scores of the next
+            // ---- matrix half: the next loads; P V of the block, the scores of the next
+            if (__builtin_expect(key0 + 2u * STEP + BK <= in, 1)) {
+                load_whole(s, vn, vsn, vraw);
+                load_whole(s, kn, ksn, kraw);
+            } else {
+                load_any(s, s.v, s.vs, key0 + STEP, vraw);
+                load_any(s, s.k, s.ks, key0 + 2u * STEP, kraw);
+            }
+            vn += step * EB;
+            kn += step * EB;
+            if constexpr (F8) {
+                vsn += step / HD;
+                ksn += step / HD;
+            }
             if (__builtin_expect(live, 1)) {
                 __builtin_amdgcn_s_setprio(1);
                 matrix<true>(vl, kl);
