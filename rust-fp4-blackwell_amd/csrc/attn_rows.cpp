@@ -93,23 +93,29 @@ uint64_t splits_of_own(uint64_t keys, uint32_t rows, uint32_t nkv)
 }
 uint64_t tiles_of(bool many, uint64_t flat) { return many ? (flat + 63) / 64 : (flat + 15) / 16; }
 
-Plan plan(bool causal, uint32_t nkv, uint32_t group, uint32_t hd, uint32_t rows, uint64_t len0, uint64_t cap1)
+Plan plan(bool causal, bool fp8, uint32_t nkv, uint32_t group, uint32_t hd, uint32_t rows, uint64_t len0, uint64_t cap1)
 {
     Plan p{};
     const uint64_t flat = (uint64_t)rows * group;
     // 16 query rows for a workgroup whose waves read keys of their own, or 64 for
     // one that stages them: the first reads and converts a key for every 16 rows
-    // and starts sooner, so few rows or keys are its.  The line is a number of
-    // scores, query heads x keys.  Measured (us, few / many): heads of 128, 400
-    // prompt rows 17.6 / 18.0 (2.6e6 scores), 512 20.1 / 19.9 (4.2e6), 700 29.7 /
-    // 25.8 (7.8e6), 64 rows over 2048 shared fp16 keys 21.0 / 25.1 (4.2e6), 4096
-    // 29.3 / 25.6 (8.4e6), 16384 83.8 / 48.8; 8 bits, 4096 25.7 / 29.7, 8192 38.4 /
-    // 35.4, 16384 67.9 / 50.9; heads of 64, 700 prompt rows 16.7 / 19.2 (7.8e6),
-    // 1024 24.3 / 23.1 (1.7e7), 64 rows over 4096 fp16 keys 20.2 / 20.1 (8.4e6).  Up
-    // to 32 rows of a KV head the second wastes half its waves (20 rows of 64 over
-    // 4096 keys 10.5 / 13.5).
+    // and starts sooner, so few rows or keys are its.  Up to 32 rows of a KV head the
+    // second wastes half its waves (20 rows of 64 over 4096 keys 12.3 / 14.9 us, few
+    // / many).  Prompts that give it a workgroup for most CUs without splits, by the
+    // scores (query heads x keys): heads of 128, 320 rows (160 workgroups) 14.6 / 15.7,
+    // 400 18.6 / 17.5 (2.6e6), 512 20.4 / 18.8, 700 29.5 / 23.8, 512 after 2048 63.1 /
+    // 50.7; heads of 64, 700 15.4 / 16.9 (7.8e6), 1024 23.8 / 22.1 (1.7e7), 512 after
+    // 2048 35.6 / 32.9.  Else splits have to be long, by the keys: 8 bits, heads of 128,
+    // 64 rows over 4096 25.3 / 29.2, 6144 32.7 / 31.3, 16384 67.6 / 47.5, 128 after 4096
+    // 32.8 / 36.7, 8192 58.6 / 52.8, 256 after 4096 53.6 / 56.7, 8192 96.9 / 82.2; of
+    // 64, 64 over 8192 30.5 / 26.3, 256 after 4096 32.9 / 40.5; fp16, which needs no
+    // conversion, 64 over 2048 21.2 / 25.1, 4096 29.1 / 26.9, 16384 83.0 / 44.8; 16 rows
+    // over 8192 (4.2e6 scores) are the first's.
     const uint64_t keys = causal ? (uint64_t)rows * (len0 - rows) + (uint64_t)rows * (rows + 1u) / 2u : (uint64_t)rows * len0;
-    p.many = flat > 32 && keys * group * nkv > (hd == 128 ? 6000000u : 12000000u);
+    const uint64_t scores = keys * group * nkv;
+    const bool full = causal && tiles_of(true, flat) * nkv >= 192u, full_scores = scores > (hd == 128 ? 2500000u : 12000000u);
+    const bool split = len0 >= (fp8 ? 6000u : 4000u) && scores > (hd == 128 ? 6000000u : 12000000u);
+    p.many = flat > 32 && (full ? full_scores : split);
     if (t_mode) p.many = t_mode == 2;
     if (len0) {
         p.tiles0 = (uint32_t)tiles_of(p.many, flat);
@@ -226,7 +232,7 @@ int causal(const char *what, hipStream_t s, uint32_t nh, uint32_t nkv, uint32_t 
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = rows; a.causal = 1; a.pos0 = pos0; a.len0 = (uint32_t)keys;
-    return run(what, plan(true, nkv, nh / nkv, hd, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
+    return run(what, plan(true, true, nkv, nh / nkv, hd, rows, keys, 0), a, true, hd, workspace, workspace_bytes, s);
 }
 
 int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint32_t nh, uint32_t nkv, uint32_t hd, const float *q, uint32_t q_rs,
@@ -254,7 +260,7 @@ int prefix_rows(const char *what, bool fp8, hipStream_t s, uint32_t batch, uint3
     a.q_rs = q_rs; a.out_rs = out_rs;
     a.n_heads = nh; a.n_kv_heads = nkv;
     a.rows = batch; a.len0 = prefix; a.cap1 = max_suffix;
-    return run(what, plan(false, nkv, nh / nkv, hd, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
+    return run(what, plan(false, fp8, nkv, nh / nkv, hd, batch, prefix, max_suffix), a, fp8, hd, workspace, workspace_bytes, s);
 }
 
 } // namespace
